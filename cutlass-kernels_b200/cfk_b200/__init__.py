@@ -14,16 +14,19 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "libcfk_b200.so")
 
-FP16, BF16, E4M3, FP32 = 0, 1, 2, 3
+FP16, BF16, E4M3, FP32, INT8 = 0, 1, 2, 3, 4
 DTYPES = {"fp16": FP16, "bf16": BF16, "e4m3": E4M3, "fp32": FP32}
 
 STATUS_NAMES = {0: "OK", 1: "INVALID_ARG", 2: "UNSUPPORTED", 3: "DESCRIPTOR", 4: "LAUNCH", 5: "NO_DRIVER",
                 6: "DEVICE_WAIT", 7: "TOO_LARGE"}
 
 EXPORTS = ["cfk_fmha_forward", "cfk_fmha_forward_static", "cfk_gemm", "cfk_fill", "cfk_convert", "cfk_device_status",
-           "cfk_last_cuda_error", "cfk_version", "cfk_selftest_umma", "cfk_umma_peak", "cfk_selftest_wait_gives_up", "cfk_selftest_wait_gives_up_static", "cfk_set_tunable", "cfk_get_tunable", "cfk_fmha_plan", "cfk_gemm_plan"]
+           "cfk_last_cuda_error", "cfk_version", "cfk_selftest_umma", "cfk_umma_peak", "cfk_selftest_wait_gives_up", "cfk_selftest_wait_gives_up_static", "cfk_set_tunable", "cfk_get_tunable", "cfk_fmha_plan", "cfk_gemm_plan",
+           "cfk_quantize_rows", "cfk_gemm_i8", "cfk_ffn_gated", "cfk_ffn_gated_backward"]
 
 TUNE_FMHA_EXP_EMU, TUNE_FMHA_GROUP_MB, TUNE_FMHA_KERNEL, TUNE_FMHA_GRID, TUNE_FMHA_SCHED = 0, 1, 2, 3, 4
+
+ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_RELU = 0, 1, 2, 3
 
 
 class FmhaArgs(C.Structure):
@@ -48,6 +51,36 @@ class GemmArgs(C.Structure):
         ("a", C.c_void_p), ("b", C.c_void_p), ("c", C.c_void_p),
         ("alpha", C.c_float), ("beta", C.c_float), ("c_row_major", C.c_int), ("iterations", C.c_int),
         ("c_src", C.c_void_p),
+    ]
+
+
+class GemmI8Args(C.Structure):
+    _fields_ = [
+        ("out_dtype", C.c_int), ("m", C.c_int), ("n", C.c_int), ("k", C.c_int),
+        ("a", C.c_void_p), ("b", C.c_void_p), ("c", C.c_void_p),
+        ("a_scale", C.c_void_p), ("b_scale", C.c_void_p), ("bias", C.c_void_p),
+        ("a_stride", C.c_int64), ("b_stride", C.c_int64), ("c_stride", C.c_int64),
+    ]
+
+
+class FfnGatedArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("out_dtype", C.c_int), ("activation", C.c_int), ("m", C.c_int), ("n", C.c_int), ("k", C.c_int),
+        ("x", C.c_void_p), ("w_gate", C.c_void_p), ("w_up", C.c_void_p),
+        ("h", C.c_void_p), ("gate", C.c_void_p), ("up", C.c_void_p),
+        ("x_scale", C.c_void_p), ("gate_scale", C.c_void_p), ("up_scale", C.c_void_p),
+        ("x_stride", C.c_int64), ("w_stride", C.c_int64), ("h_stride", C.c_int64), ("pre_stride", C.c_int64),
+    ]
+
+
+class FfnGatedBackwardArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("activation", C.c_int), ("m", C.c_int), ("n", C.c_int), ("k", C.c_int),
+        ("dh", C.c_void_p), ("x", C.c_void_p), ("w_gate", C.c_void_p), ("w_up", C.c_void_p), ("gate", C.c_void_p),
+        ("up", C.c_void_p), ("dgate", C.c_void_p), ("dup", C.c_void_p), ("dx", C.c_void_p), ("dw_gate", C.c_void_p),
+        ("dw_up", C.c_void_p),
+        ("dh_stride", C.c_int64), ("x_stride", C.c_int64), ("w_stride", C.c_int64), ("pre_stride", C.c_int64),
+        ("dpre_stride", C.c_int64), ("dx_stride", C.c_int64), ("dw_stride", C.c_int64),
     ]
 
 
@@ -89,6 +122,11 @@ class CfkLib:
         L.cfk_fill.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_int64, C.c_int, C.c_float, C.c_float,
                                C.c_void_p]
         L.cfk_convert.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_void_p]
+        L.cfk_quantize_rows.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_int,
+                                        C.c_void_p]
+        L.cfk_gemm_i8.argtypes = [C.POINTER(GemmI8Args), C.c_void_p]
+        L.cfk_ffn_gated.argtypes = [C.POINTER(FfnGatedArgs), C.c_void_p]
+        L.cfk_ffn_gated_backward.argtypes = [C.POINTER(FfnGatedBackwardArgs), C.c_void_p]
         L.cfk_device_status.argtypes = [C.POINTER(C.c_int)]
         L.cfk_last_cuda_error.restype = C.c_char_p
         L.cfk_selftest_umma.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p] + [C.c_int] * 5 + [C.c_void_p]
@@ -141,6 +179,37 @@ class CfkLib:
              c_src=None, stream=None) -> None:
         rc = self.lib.cfk_gemm(GemmArgs(dtype, m, n, k, l, _ptr(a), _ptr(b), _ptr(c), alpha, beta,
                                         1 if c_row_major else 0, iterations, _ptr(c_src)), stream)
+        if rc:
+            raise CfkError(rc, self.last_error())
+
+    # Feed-forward operators; strides are in elements between rows, 0 = packed (include/cfk_b200.h).
+    def quantize_rows(self, src, dst, scale, *, src_dtype, rows, cols, src_stride=0, dst_stride=0, stream=None) -> None:
+        rc = self.lib.cfk_quantize_rows(_ptr(src), src_dtype, src_stride, _ptr(dst), dst_stride, _ptr(scale), rows, cols, stream)
+        if rc:
+            raise CfkError(rc, self.last_error())
+
+    def gemm_i8(self, a, b, c, *, m, n, k, out_dtype, a_scale, b_scale, bias=None, a_stride=0, b_stride=0, c_stride=0,
+                stream=None) -> None:
+        rc = self.lib.cfk_gemm_i8(GemmI8Args(out_dtype, m, n, k, _ptr(a), _ptr(b), _ptr(c), _ptr(a_scale), _ptr(b_scale),
+                                             _ptr(bias), a_stride, b_stride, c_stride), stream)
+        if rc:
+            raise CfkError(rc, self.last_error())
+
+    def ffn_gated(self, x, w_gate, w_up, h, *, dtype, out_dtype, activation, m, n, k, gate=None, up=None, x_scale=None,
+                  gate_scale=None, up_scale=None, x_stride=0, w_stride=0, h_stride=0, pre_stride=0, stream=None) -> None:
+        rc = self.lib.cfk_ffn_gated(
+            FfnGatedArgs(dtype, out_dtype, activation, m, n, k, _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(h), _ptr(gate), _ptr(up),
+                         _ptr(x_scale), _ptr(gate_scale), _ptr(up_scale), x_stride, w_stride, h_stride, pre_stride), stream)
+        if rc:
+            raise CfkError(rc, self.last_error())
+
+    def ffn_gated_backward(self, dh, x, w_gate, w_up, gate, up, dgate, dup, *, dtype, activation, m, n, k, dx=None,
+                           dw_gate=None, dw_up=None, dh_stride=0, x_stride=0, w_stride=0, pre_stride=0, dpre_stride=0,
+                           dx_stride=0, dw_stride=0, stream=None) -> None:
+        rc = self.lib.cfk_ffn_gated_backward(
+            FfnGatedBackwardArgs(dtype, activation, m, n, k, _ptr(dh), _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(gate), _ptr(up),
+                                 _ptr(dgate), _ptr(dup), _ptr(dx), _ptr(dw_gate), _ptr(dw_up), dh_stride, x_stride, w_stride,
+                                 pre_stride, dpre_stride, dx_stride, dw_stride), stream)
         if rc:
             raise CfkError(rc, self.last_error())
 

@@ -78,7 +78,7 @@ int encode_tiled(CUtensorMap* map, int dtype, int rank, const void* base, const 
   if (!fn) return CFK_ERR_NO_DRIVER;
   CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   if (dtype == CFK_BF16) dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  else if (dtype == CFK_E4M3) dt = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  else if (dtype == CFK_E4M3 || dtype == CFK_INT8) dt = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   else if (dtype == CFK_FP32) dt = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   cuuint64_t gd[5];
   cuuint64_t gs[4];

@@ -236,10 +236,10 @@ __host__ __device__ __forceinline__ uint64_t make_smem_desc(uint32_t saddr, uint
 // Advance the start address of a descriptor by `bytes` (a multiple of 16).
 __device__ __forceinline__ uint64_t desc_advance(uint64_t d, uint32_t bytes) { return d + (bytes >> 4); }
 
-// Instruction descriptor (32 bit) for kind::f16 / kind::tf32 / kind::f8f6f4.
-//   c_format: 0 f16, 1 f32.  a/b format: kind::f16 -> 0 f16, 1 bf16; kind::f8f6f4 -> 0 e4m3, 1 e5m2.
+// Instruction descriptor (32 bit) for kind::f16 / kind::tf32 / kind::f8f6f4 / kind::i8.
+//   c_format: 0 f16, 1 f32, 2 s32.  a/b format: kind::f16 -> 0 f16, 1 bf16; kind::f8f6f4 -> 0 e4m3, 1 e5m2; kind::i8 -> 1 s8.
 //   major: 0 = K-major, 1 = MN-major.
-constexpr uint32_t kFmtF16 = 0, kFmtBF16 = 1, kFmtE4M3 = 0;
+constexpr uint32_t kFmtF16 = 0, kFmtBF16 = 1, kFmtE4M3 = 0, kFmtS8 = 1;
 __host__ __device__ constexpr uint32_t make_idesc(uint32_t c_format, uint32_t a_format, uint32_t b_format,
                                                   uint32_t a_major, uint32_t b_major, uint32_t M, uint32_t N) {
   return (c_format << 4) | (a_format << 7) | (b_format << 10) | (a_major << 15) | (b_major << 16) |
@@ -468,6 +468,19 @@ __device__ __forceinline__ void umma_ss_pair_tf32(uint32_t d_tmem, uint64_t a_de
       "@q tcgen05.mma.cta_group::2.kind::tf32 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
+}
+// 8-bit integers (kind::i8): 32 elements (32 bytes) of reduction per instruction, exact sums in 32-bit integers.
+template <bool PAIR>
+__device__ __forceinline__ void umma_ss_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate, uint32_t leader) {
+  if constexpr (PAIR)
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
 }
 // Move registers between warpgroups (executed by every warp of a warpgroup).
 template <int N>

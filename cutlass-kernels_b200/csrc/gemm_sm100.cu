@@ -35,6 +35,7 @@
 #include <utility>
 
 #include "common.cuh"
+#include "gemm_tiles.cuh"
 #include "host_util.h"
 
 namespace cfk {
@@ -76,22 +77,6 @@ struct GemmCfg {
   static_assert(UNITS * UNITB <= NSTAGE * (XB + YB), "split: the accumulator is handed over in the ring");
   static_assert(8 * (2 * NSTAGE + 8) + 8 <= 256, "barrier block overflows");
 };
-constexpr int kGemmBand = 8;
-
-__device__ __forceinline__ void tile_coords(int tile, int tiles_r, int tiles_c, int& tr, int& tc, int& batch) {
-  const int per_batch = tiles_r * tiles_c;
-  batch = tile / per_batch;
-  int t = tile - batch * per_batch;
-  const int band_tiles = kGemmBand * tiles_c;
-  const int band = t / band_tiles;
-  const int first_r = band * kGemmBand;
-  const int rows_in_band = (tiles_r - first_r) < kGemmBand ? (tiles_r - first_r) : kGemmBand;
-  t -= band * band_tiles;
-  tr = first_r + t % rows_in_band;
-  tc = t / rows_in_band;
-  if (band & 1) tc = tiles_c - 1 - tc;   // back and forth: a band starts on the Y panels the band before it ended on
-}
-
 // The beta term.  32 columns of a row of the source matrix, from element `at` on, `cols` of which exist, are read ahead of
 // their use: a read takes about a microsecond, and the epilogue would otherwise wait for one per 32 columns.
 struct SourceRow { uint4 x[8]; };     // 8 pieces of 4 fp32, or 4 of 8 16-bit values
@@ -134,10 +119,6 @@ __device__ __forceinline__ void add_source(float (&v)[32], const GemmParams& p, 
     }
   }
 }
-__device__ __forceinline__ uint32_t pack_out(bool bf16, float lo, float hi) {
-  return bf16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
-}
-
 template <int TN>
 __global__ void __launch_bounds__(192, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_y,

@@ -54,7 +54,13 @@ int* device_status_block(int* err);
 // Device address of the fixed scratch array that cfk_fmha_forward_static uses (fmha_static.cu); allocates nothing.
 int* static_scratch_for_current_device(int* err);
 
-inline int dtype_size(int dt) { return dt == CFK_E4M3 ? 1 : (dt == CFK_FP32 ? 4 : 2); }
+inline int dtype_size(int dt) { return dt == CFK_E4M3 || dt == CFK_INT8 ? 1 : (dt == CFK_FP32 ? 4 : 2); }
+
+// Rows of a matrix as the feed-forward operators take them: at multiples of 16 bytes, not overlapping, within what a tensor map's
+// stride field holds (2^40 bytes for all rows).
+inline bool rows_ok(const void* base, int dt, int64_t cols, int64_t stride) {
+  return ((uintptr_t)base & 15u) == 0 && stride >= cols && stride < (int64_t)1 << 31 && (stride * dtype_size(dt)) % 16 == 0;
+}
 
 // Generic tiled descriptor.  dims/box are innermost first; strides_bytes has rank-1 entries.
 // Returns CFK_OK, CFK_ERR_NO_DRIVER or CFK_ERR_DESCRIPTOR.

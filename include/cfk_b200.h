@@ -20,7 +20,8 @@ extern "C" {
 
 typedef struct CUstream_st* cfk_stream_t; /* == cudaStream_t */
 
-enum cfk_dtype { CFK_FP16 = 0, CFK_BF16 = 1, CFK_E4M3 = 2, CFK_FP32 = 3 };
+enum cfk_dtype { CFK_FP16 = 0, CFK_BF16 = 1, CFK_E4M3 = 2, CFK_FP32 = 3,
+                 CFK_INT8 = 4 /* cfk_ffn_gated only; cfk_quantize_rows and cfk_gemm_i8 imply it */ };
 
 enum cfk_status {
   CFK_OK = 0,
@@ -149,6 +150,108 @@ int cfk_gemm(const cfk_gemm_args* args, cfk_stream_t stream);
  */
 int cfk_fmha_plan(const cfk_fmha_args* args, int plan[4]);
 int cfk_gemm_plan(const cfk_gemm_args* args, int plan[3]);
+
+/*
+ * Feed-forward operators: 8-bit integer products and the gated block.  No counterpart in the reference, whose programs
+ * stop at attention and one GEMM; they take the place that cfk_gemm has for plain layers.
+ *
+ * All matrices are row-major with one row per token (activations) or per output channel (weights, as in cfk_gemm's B).
+ * A *_stride is the distance of two rows in elements, 0 = packed; it is at least the row's length.  Rows of what the tensor
+ * core reads (operands) and of every output of cfk_gemm_i8, cfk_ffn_gated and cfk_ffn_gated_backward start at multiples of 16
+ * bytes: base pointers are 16-byte aligned and stride times element size is a multiple of 16, else CFK_ERR_INVALID_ARG.
+ * The lengths themselves are free: any m, n, k >= 1.  Nothing is read or written behind the end of a row.  Outputs overlap no
+ * input and no other output, unless a comment allows it.  Sums are exact (integers) or fp32; results are rounded once.
+ * Pointers and stream belong to the current device.  No workspace but the status block (cfk_device_status reports a wait
+ * that gave up, codes 211-216 and 221-224); calls can be captured.  Results do not depend on timing.  Which kernel a call
+ * runs depends on its sizes and types (and, with it, the order of fp32 sums); integer sums do not depend on it.
+ */
+
+/*
+ * Symmetric 8-bit quantisation with one scale per row (a token's activations, a channel's weights):
+ *   scale[i] = max_j |x[i][j]| / 127 (fp32),  q[i][j] = x[i][j] / scale[i] (fp32), rounded to nearest even, within -127..127.
+ * A row whose scale is 0 (all zeros, or underflow) gets q = 0 and scale = 0.  A row that holds an infinity or a NaN gets q = 0
+ * and scale = NaN, so that what is computed from it shows.  src_dtype: FP16, BF16 or FP32; rows of src and dst start at
+ * multiples of 16 bytes.  x itself is not written.
+ */
+int cfk_quantize_rows(const void* src, int src_dtype, int64_t src_stride, void* dst, int64_t dst_stride, float* scale,
+                      int rows, int cols, cfk_stream_t stream);
+
+/*
+ * C[i][j] = a_scale[i] * b_scale[j] * sum_k A[i][k] B[j][k]  (+ bias[j]), A [m][k] and B [n][k] signed 8-bit integers.
+ * The sums are 32-bit integers and exact; k above 131071 (2^31 / 128^2) is refused, CFK_ERR_UNSUPPORTED.
+ */
+typedef struct cfk_gemm_i8_args {
+  int out_dtype;               /* C: FP16, BF16 or FP32 */
+  int m, n, k;
+  const void* a;               /* [m][k] tokens */
+  const void* b;               /* [n][k] weights */
+  void* c;                     /* [m][n] */
+  const float* a_scale;        /* [m] */
+  const float* b_scale;        /* [n] */
+  const float* bias;           /* [n] or null */
+  int64_t a_stride, b_stride, c_stride;
+} cfk_gemm_i8_args;
+
+int cfk_gemm_i8(const cfk_gemm_i8_args* args, cfk_stream_t stream);
+
+/* GELU: x * Phi(x) with the normal distribution; GELU_TANH: its tanh form, 0.5 x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))). */
+enum cfk_activation { CFK_ACT_SILU = 0, CFK_ACT_GELU = 1, CFK_ACT_GELU_TANH = 2, CFK_ACT_RELU = 3 };
+
+/*
+ * Gated feed-forward block up to its product, in one kernel:
+ *   gate = x Wg^T,  up = x Wu^T,  h = act(gate) * up.
+ * The projection back is a cfk_gemm or cfk_gemm_i8 of h.  Weights that are stored as one [2n][k] matrix are passed as two
+ * pointers into it.  With gate and up given (both or neither) the pre-activations are written too, as the backward pass
+ * needs them; h is computed from the unrounded ones.
+ */
+typedef struct cfk_ffn_gated_args {
+  int dtype;                   /* x, w_gate, w_up: FP16, BF16 or INT8 */
+  int out_dtype;               /* h, gate, up: FP16 or BF16; equal to dtype for 16-bit inputs */
+  int activation;              /* cfk_activation */
+  int m, n, k;                 /* tokens, width of the block, width of the model */
+  const void* x;               /* [m][k] */
+  const void* w_gate;          /* [n][k] */
+  const void* w_up;            /* [n][k] */
+  void* h;                     /* [m][n] */
+  void* gate;                  /* [m][n] or null */
+  void* up;                    /* [m][n] or null */
+  const float* x_scale;        /* [m], INT8 only (null otherwise) */
+  const float* gate_scale;     /* [n], INT8 only */
+  const float* up_scale;       /* [n], INT8 only */
+  int64_t x_stride, w_stride /* w_gate and w_up */, h_stride, pre_stride /* gate and up */;
+} cfk_ffn_gated_args;
+
+int cfk_ffn_gated(const cfk_ffn_gated_args* args, cfk_stream_t stream);
+
+/*
+ * Gradients of cfk_ffn_gated for 16-bit types, from dh = dL/dh and the gate and up that the forward call kept:
+ *   dgate = dh * up * act'(gate),  dup = dh * act(gate),
+ *   dx = dgate Wg + dup Wu,  dw_gate = dgate^T x,  dw_up = dup^T x.
+ * dgate and dup are outputs that the products read: they are rounded to dtype, as the tensor core takes them, which adds to
+ * each product an error of the size of its own rounding.  dgate may be the buffer of gate (or dup that of up) with the same
+ * stride, which saves their memory.  Three launches; dx null leaves its product out, dw_gate and dw_up (both or neither) theirs.
+ * act'(0) of RELU is 0.
+ */
+typedef struct cfk_ffn_gated_backward_args {
+  int dtype;                   /* all matrices: FP16 or BF16 */
+  int activation;
+  int m, n, k;
+  const void* dh;              /* [m][n] */
+  const void* x;               /* [m][k] */
+  const void* w_gate;          /* [n][k] */
+  const void* w_up;            /* [n][k] */
+  const void* gate;            /* [m][n] */
+  const void* up;              /* [m][n] */
+  void* dgate;                 /* [m][n] */
+  void* dup;                   /* [m][n] */
+  void* dx;                    /* [m][k] or null */
+  void* dw_gate;               /* [n][k] or null */
+  void* dw_up;                 /* [n][k] or null */
+  int64_t dh_stride, x_stride, w_stride, pre_stride /* gate, up */, dpre_stride /* dgate, dup */, dx_stride,
+      dw_stride /* dw_gate, dw_up */;
+} cfk_ffn_gated_backward_args;
+
+int cfk_ffn_gated_backward(const cfk_ffn_gated_backward_args* args, cfk_stream_t stream);
 
 /*
  * Device-side random fills, element i depends only on (seed, first_index + i).
