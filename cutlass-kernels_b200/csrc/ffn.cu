@@ -1,6 +1,8 @@
 // Entry points of the feed-forward operators (include/cfk_b200.h): argument checks, descriptors and choice of kernel, and the
 // elementwise part of the gated block's backward pass.
+#include <cmath>
 #include <cstring>
+#include <utility>
 
 #include "common.cuh"
 #include "element_io.cuh"
@@ -72,58 +74,227 @@ static cudaError_t launch_gate_grad(const cfk_ffn_gated_backward_args* a, int64_
                            (const uint16_t*)a->up, (uint16_t*)a->dgate, (uint16_t*)a->dup, dh_s, pre_s, dpre_s, a->n, nvec, total);
 }
 
-// ---- descriptors ------------------------------------------------------------------------------------------------------------
-// A matrix of `rows` rows of `cols` elements, read or written in boxes of 128 bytes x `box_rows` rows.
-static int encode_rows(CUtensorMap* map, int dtype, const void* base, int rows, int cols, int64_t stride, int box_rows) {
-  const uint64_t esz = (uint64_t)dtype_size(dtype);
-  const uint64_t dims[3] = {(uint64_t)cols, (uint64_t)rows, 1};
-  const uint64_t strides[2] = {(uint64_t)stride * esz, (uint64_t)stride * esz};
-  const uint32_t box[3] = {(uint32_t)(128 / esz), (uint32_t)box_rows, 1};
-  return encode_tiled(map, dtype, 3, base, dims, strides, box, 128);
+// ---- cuts -------------------------------------------------------------------------------------------------------------------
+// Which kernel and which tiles follows from estimates of its time, in us, whose constants are fits to a sweep of 240 shapes (1 to
+// 3000 tokens, widths 128 to 11264 and 8192) x all cuts: root mean square error 7 to 13 %, and the cut they choose is on average
+// within 2 % of the best one measured, at worst 35 %.
+constexpr int kPairs = kSMs / 2;
+
+static bool is_gated(int mode) { return mode == kGated16 || mode == kGatedI8; }
+static int k_blocks(int mode, int reduce) {
+  const int kb = mode == kProductI8 || mode == kGatedI8 ? 128 : 64;
+  return (reduce + kb - 1) / kb;
 }
 
+// Clusters of 1, 2, 3, 4, 6 and 8 CTAs that are resident at once, with one and with two CTAs per SM, as
+// cudaOccupancyMaxActiveClusters answers on B200.
+constexpr int kSplits[6] = {1, 2, 3, 4, 6, 8};
+constexpr int kResident[2][6] = {{148, 74, 45, 33, 22, 15}, {296, 148, 93, 71, 45, 33}};
+
+// The kernel for few tokens: the longest of what a CTA takes for its k-blocks (a round of the ring, or what an SM takes in), the
+// tiles' traffic from L2 and the weights' from DRAM; then the epilogue and the exchange of a split.  One CTA per SM with the deepest
+// ring where the clusters fit that way: one gated token of 11264 x 4096 bf16 32.0 us against 36.2 with half of it.
+static float plan_few(int mode, int rows, int cols, int reduce, FewPlan* best) {
+  const int nw = few_weights(mode), nkb = k_blocks(mode, reduce) * (mode == kGrad ? 2 : 1);
+  const float round = mode == kGrad ? 0.25f : 0.21f, intake = mode == kGrad ? 125.f : 155.f;      // us, KB per us
+  const int tiles_ch = (cols + 127) / 128;
+  float best_t = 0.f;
+  for (int tt = 16; tt <= 256 / nw; tt *= 2) {
+    if (tt > 16 && tt >= 2 * rows) break;
+    const int stage = nw * 16384 + tt * 128, half = (kFewSmemHalf - kFewHead) / stage, full = (kFewSmemFull - kFewHead) / stage;
+    const int tiles_tok = (rows + tt - 1) / tt, ntok = rows < tt ? rows : tt;
+    const long long tiles = (long long)tiles_ch * tiles_tok;
+    if (tiles > 65536) continue;
+    const float l2 = (float)tiles * (float)nkb * (float)stage / 13.5e6f;
+    const float dram = (float)tiles_ch * (float)nkb * (float)(nw * 16384) / 5.2e6f;
+    for (int i = 0; i < 6; ++i) {
+      const int s = kSplits[i];
+      if (s > nkb) break;
+      const bool two = half >= 3 && tiles > kResident[0][i];
+      const int resident = kResident[two][i], waves = (int)((tiles + resident - 1) / resident);
+      const float live = (float)((tiles < resident ? (int)tiles : resident) * s);
+      const float share = two && live > (float)kSMs ? live / (float)kSMs : 1.f;                   // CTAs that an SM feeds
+      const float chain = (float)(waves * ((nkb + s - 1) / s)) * fmaxf(round, share * (float)stage / 1024.f / intake);
+      const float finish = 0.02f * (float)(nw * ntok) / (float)s + (s > 1 ? 2.0f + 0.022f * (float)(nw * ntok) : 0.f);
+      const float t = 2.5f + fmaxf(chain, fmaxf(l2, dram)) + finish + (float)(waves - 1) * (2.5f + finish);
+      if (best_t == 0.f || t < best_t) {
+        const int stages = two ? half : full;
+        best_t = t;
+        *best = FewPlan{tt, s, stages < kFewMaxStages ? stages : kFewMaxStages, tiles_ch, tiles_tok};
+      }
+    }
+  }
+  return best_t;
+}
+
+static long long set_width(PairJob* j, bool gated, int bn) {
+  j->bn = bn;
+  j->tiles_r = (j->rows + 255) / 256;
+  j->tiles_c = (j->cols + (gated ? bn : 2 * bn) - 1) / (gated ? bn : 2 * bn);
+  return (long long)j->tiles_r * j->tiles_c * j->batches;
+}
+// Widths of the tiles of a launch on CTA pairs, and how the pairs share two lists of them.  MN-major k-blocks take as long whatever the
+// width (four loads of 64 x 64).  With one turn over both lists, whatever a pair had of the first, 12158 tokens of 768 x 1472 took
+// 116 us for what sharing does in 83.
+static float plan_pairs(int mode, PairPlan* plan) {
+  static const int kWidth[3] = {128, 96, 64};
+  static const float kBlock[2][3] = {{0.32f, 0.25f, 0.205f}, {0.305f, 0.295f, 0.29f}};
+  const bool gated = is_gated(mode);
+  PairPlan best = *plan;
+  float best_t = 0.f;
+  for (int w = 0; w < (plan->jobs > 1 ? 9 : 3); ++w) {
+    const int width[2] = {w % 3, w / 3};
+    long long tiles[2] = {0, 0};
+    float each[2] = {0.f, 0.f}, last[2] = {0.f, 0.f}, bytes = 0.f;
+    for (int i = 0; i < plan->jobs; ++i) {
+      PairJob& j = plan->job[i];
+      const int bn = kWidth[width[i]], nkb = k_blocks(mode, j.reduce) * (mode == kGrad && j.kind == 0 ? 2 : 1);
+      tiles[i] = set_width(&j, gated, bn);
+      last[i] = 1.15f * (float)bn / 128.f;
+      each[i] = 1.5f + fmaxf((float)nkb * kBlock[mode == kGrad][width[i]], last[i]);
+      bytes += (float)tiles[i] * (float)nkb * (float)(32768 + 2 * bn * 128);
+    }
+    const long long all = tiles[0] + tiles[1], pairs = all < kPairs ? all : kPairs;
+    const long long most = tiles[0] / pairs, more = tiles[0] % pairs;      // `more` pairs have most + 1 tiles of the first list
+    long long share = 0;
+    float longest = (float)(most + (more > 0)) * each[0] + last[0];
+    if (tiles[1] > 0) {
+      // the least that leaves the other pairs no later than those with one tile more, or one less than that
+      const float even = ((float)tiles[1] * each[1] - (float)(pairs - more) * each[0]) / ((float)pairs * each[1]);
+      const long long from = even > 0.f ? (long long)even : 0, limit = more > 0 ? tiles[1] / more : 0;
+      longest = 0.f;
+      for (long long x = from; x <= from + 1; ++x) {
+        const long long s = x < limit ? x : limit, rest = tiles[1] - more * s, others = (rest + pairs - more - 1) / (pairs - more);
+        const float a = more > 0 ? (float)(most + 1) * each[0] + (float)s * each[1] + (s > 0 ? last[1] : last[0]) : 0.f;
+        const float b = (float)most * each[0] + (float)others * each[1] + (others > 0 ? last[1] : last[0]);
+        if (longest == 0.f || fmaxf(a, b) < longest) { longest = fmaxf(a, b); share = s; }
+      }
+    }
+    const float t = 2.5f + fmaxf(longest, bytes / 12.5e6f);
+    if (best_t == 0.f || t < best_t) {
+      best_t = t;
+      best = *plan;
+      best.pairs = (int)pairs;
+      best.share = (int)share;
+    }
+  }
+  *plan = best;
+  return best_t;
+}
+static bool too_many_tiles(const PairPlan& plan) {
+  long long n = 0;
+  for (int i = 0; i < plan.jobs; ++i) n += (long long)plan.job[i].tiles_r * plan.job[i].tiles_c * plan.job[i].batches;
+  return n > 0x7fffffffLL - kPairs;
+}
+
+// A forward product: few.tt = 0, or the pairs are not used.
+struct ProductPlan { FewPlan few; PairPlan pair; };
+static ProductPlan plan_product(int mode, int rows, int cols, int reduce) {
+  ProductPlan plan;
+  std::memset(&plan, 0, sizeof(plan));
+  plan.pair.jobs = 1;
+  PairJob& j = plan.pair.job[0];
+  j.rows = rows; j.cols = cols; j.reduce = reduce; j.batches = 1;
+  const float few = plan_few(mode, rows, cols, reduce, &plan.few), pair = plan_pairs(mode, &plan.pair);
+  if (few == 0.f || pair < few) plan.few.tt = 0;
+  return plan;
+}
+// The backward products: dx in the kernel for few tokens (few.tt > 0) or on pairs, there in one launch with the weights' gradients.
+static ProductPlan plan_backward(const cfk_ffn_gated_backward_args* a) {
+  ProductPlan plan;
+  std::memset(&plan, 0, sizeof(plan));
+  PairJob dx, dw;
+  std::memset(&dx, 0, sizeof(dx));
+  dw = dx;
+  dx.rows = a->m; dx.cols = a->k; dx.reduce = a->n; dx.batches = 1;
+  dw.kind = 1; dw.rows = a->n; dw.cols = a->k; dw.reduce = a->m; dw.batches = 2;
+  PairPlan alone = plan.pair, both = plan.pair;
+  float t_alone = 0.f;
+  if (a->dw_gate) {
+    alone.jobs = 1;
+    alone.job[0] = dw;
+    t_alone = plan_pairs(kGrad, &alone);
+  }
+  plan.pair = alone;
+  if (!a->dx) return plan;
+  both.jobs = a->dw_gate ? 2 : 1;
+  both.job[0] = dx;
+  both.job[1] = dw;
+  if (both.jobs == 2 && k_blocks(kGrad, a->m) > 2 * k_blocks(kGrad, a->n)) std::swap(both.job[0], both.job[1]);   // longest tiles first
+  const float few = plan_few(kGrad, a->m, a->k, a->n, &plan.few), t_both = plan_pairs(kGrad, &both);
+  if (few == 0.f || t_both < few + t_alone) {
+    plan.few.tt = 0;
+    plan.pair = both;
+  }
+  return plan;
+}
+
+// ---- descriptors ------------------------------------------------------------------------------------------------------------
 struct Matrix {
   const void* base;
   int dtype, rows, cols;
   int64_t stride;
 };
-static int encode(CUtensorMap* map, const Matrix& m, int box_rows) {
-  return encode_rows(map, m.dtype, m.base, m.rows, m.cols, m.stride, box_rows);
+// Read or written in boxes of `box_bytes` (which is the swizzle too) x `box_rows` rows.
+static int encode(CUtensorMap* map, const Matrix& m, int box_rows, int box_bytes = 128) {
+  const uint64_t esz = (uint64_t)dtype_size(m.dtype);
+  const uint64_t dims[3] = {(uint64_t)m.cols, (uint64_t)m.rows, 1};
+  const uint64_t strides[2] = {(uint64_t)m.stride * esz, (uint64_t)m.stride * esz};
+  const uint32_t box[3] = {(uint32_t)(box_bytes / esz), (uint32_t)box_rows, 1};
+  return encode_tiled(map, m.dtype, 3, m.base, dims, strides, box, box_bytes);
 }
 
-// A product's operands and results as matrices; unused ones have a null base.
+// Operands and results as in ProductMaps; unused ones have a null base.
 struct ProductCall {
-  Matrix x[2], y[2], d[3];
+  Matrix x[2], y[3], d[3];
   ProductParams p;
 };
 
-template <int MODE>
-static int run_product(const ProductCall& c, cudaStream_t stream) {
-  constexpr bool GATED = MODE == kGated16 || MODE == kGatedI8;
-  ProductParams p = c.p;
+static int prepare_results(const ProductCall& c, ProductParams* p) {
   int rc = CFK_OK;
-  p.status = device_status_block(&rc);
-  if (!p.status) return rc;
+  p->status = device_status_block(&rc);
+  for (int i = 0; i < 3; ++i) {
+    p->d[i] = const_cast<void*>(c.d[i].base);
+    p->d_stride[i] = c.d[i].stride;
+  }
+  return rc;
+}
+
+template <int MODE>
+static int run_few(const ProductCall& c, const FewPlan& few, cudaStream_t stream) {
+  ProductParams p = c.p;
   ProductMaps maps;
   std::memset(&maps, 0, sizeof(maps));
-  // K-major operands land as 128 rows of a k-block, MN-major ones as spans of 64 columns of its 64 rows
-  for (int i = 0; i < 2; ++i) {
-    if (c.x[i].base && (rc = encode(&maps.x[i], c.x[i], MODE == kGradW ? 64 : 128))) return rc;
-    if (c.y[i].base && (rc = encode(&maps.y[i], c.y[i], MODE == kGradX || MODE == kGradW ? 64 : 128))) return rc;
+  int rc = prepare_results(c, &p);
+  for (int i = 0; i < 2 && rc == CFK_OK; ++i) {
+    if (c.x[i].base) rc = encode(&maps.x[i], c.x[i], few.tt);
+    if (rc == CFK_OK && c.y[i].base) rc = encode(&maps.y[i], c.y[i], MODE == kGrad ? 64 : 128);
   }
-  p.whole = p.cols & ~(16 / dtype_size(p.out) - 1);
-  for (int i = 0; i < 3; ++i) {
-    if (!c.d[i].base) continue;
-    Matrix d = c.d[i];
-    d.cols = p.whole;
-    if (d.cols > 0 && (rc = encode(&maps.d[i], d, 128))) return rc;
-    p.d[i] = const_cast<void*>(d.base);
-    p.d_stride[i] = d.stride;
+  return rc ? rc : launch_few_product<MODE>(maps, p, few, stream);
+}
+
+template <int MODE>
+static int run_pairs(const ProductCall& c, const PairPlan& plan, cudaStream_t stream) {
+  ProductParams p = c.p;
+  ProductMaps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  int rc = prepare_results(c, &p);
+  for (int i = 0; i < 2 && rc == CFK_OK; ++i)
+    if (c.x[i].base) rc = encode(&maps.x[i], c.x[i], MODE == kGrad ? 64 : 128);
+  for (int i = 0; i < 3 && rc == CFK_OK; ++i) {
+    if (c.y[i].base) rc = encode(&maps.y[i], c.y[i], MODE == kGrad ? 64 : plan.job[0].bn);
+    Matrix d = c.d[i];         // up to the last whole 16 bytes of a row (ffn_pair_sm100.cuh, store_rest)
+    d.cols &= ~(16 / dtype_size(d.dtype) - 1);
+    if (rc == CFK_OK && d.base && d.cols > 0) rc = encode(&maps.d[i], d, 128, 32 * dtype_size(d.dtype));
   }
-  p.tiles_r = (p.rows + 255) / 256;
-  p.tiles_c = GATED ? (p.cols + 127) / 128 : (p.cols + 255) / 256;
-  if ((long long)p.tiles_r * p.tiles_c * p.batches > 0x7fffffffLL - 1024) return CFK_ERR_UNSUPPORTED;
-  return launch_pair_product<MODE>(maps, p, stream);
+  return rc ? rc : launch_pair_product<MODE>(maps, p, plan, stream);
+}
+
+template <int MODE>
+static int run_product(const ProductCall& c, cudaStream_t stream) {
+  const ProductPlan plan = plan_product(MODE, c.p.rows, c.p.cols, c.p.reduce);
+  if (plan.few.tt > 0) return run_few<MODE>(c, plan.few, stream);
+  return too_many_tiles(plan.pair) ? CFK_ERR_UNSUPPORTED : run_pairs<MODE>(c, plan.pair, stream);
 }
 
 static int64_t packed(int64_t stride, int cols) { return stride == 0 ? cols : stride; }
@@ -150,7 +321,7 @@ extern "C" int cfk_gemm_i8(const cfk_gemm_i8_args* a, cfk_stream_t stream) {
       !rows_ok(a->c, a->out_dtype, a->n, c.d[0].stride))
     return CFK_ERR_INVALID_ARG;
   if (a->k > kMaxI8Reduction) return CFK_ERR_UNSUPPORTED;
-  c.p.rows = a->m; c.p.cols = a->n; c.p.reduce = a->k; c.p.batches = 1;
+  c.p.rows = a->m; c.p.cols = a->n; c.p.reduce = a->k;
   c.p.out = a->out_dtype;
   c.p.row_scale = a->a_scale; c.p.col_scale = a->b_scale; c.p.bias = a->bias;
   return run_product<kProductI8>(c, (cudaStream_t)stream);
@@ -182,7 +353,7 @@ extern "C" int cfk_ffn_gated(const cfk_ffn_gated_args* a, cfk_stream_t stream) {
   if (a->gate && (!rows_ok(a->gate, a->out_dtype, a->n, pre_stride) || !rows_ok(a->up, a->out_dtype, a->n, pre_stride)))
     return CFK_ERR_INVALID_ARG;
   if (i8 && a->k > kMaxI8Reduction) return CFK_ERR_UNSUPPORTED;
-  c.p.rows = a->m; c.p.cols = a->n; c.p.reduce = a->k; c.p.batches = 1;
+  c.p.rows = a->m; c.p.cols = a->n; c.p.reduce = a->k;
   c.p.bf16 = a->dtype == CFK_BF16; c.p.out = a->out_dtype;
   c.p.act = a->activation; c.p.keep = a->gate != nullptr;
   c.p.row_scale = a->x_scale; c.p.col_scale = a->gate_scale; c.p.col_scale2 = a->up_scale;
@@ -210,26 +381,25 @@ extern "C" int cfk_ffn_gated_backward(const cfk_ffn_gated_backward_args* a, cfk_
   if ((long long)a->m * ((a->n + 7) / 8) > 0xffffff00LL) return CFK_ERR_UNSUPPORTED;
   const cudaStream_t st = (cudaStream_t)stream;
 
-  ProductCall gx, gw;
-  std::memset(&gx, 0, sizeof(gx));
-  const Matrix dgate = {a->dgate, dt, a->m, a->n, dpre_s}, dup = {a->dup, dt, a->m, a->n, dpre_s};
-  gx.x[0] = dgate; gx.x[1] = dup;
-  gx.p.bf16 = dt == CFK_BF16; gx.p.out = dt;
-  gw = gx;
-  gx.y[0] = {a->w_gate, dt, a->n, a->k, w_s};
-  gx.y[1] = {a->w_up, dt, a->n, a->k, w_s};
-  gx.d[0] = {a->dx, dt, a->m, a->k, dx_s};
-  gx.p.rows = a->m; gx.p.cols = a->k; gx.p.reduce = a->n; gx.p.batches = 1;
-  gw.y[0] = {a->x, dt, a->m, a->k, x_s};
-  gw.d[0] = {a->dw_gate, dt, a->n, a->k, dw_s};
-  gw.d[1] = {a->dw_up, dt, a->n, a->k, dw_s};
-  gw.p.rows = a->n; gw.p.cols = a->k; gw.p.reduce = a->m; gw.p.batches = 2;
+  ProductCall c;
+  std::memset(&c, 0, sizeof(c));
+  c.x[0] = {a->dgate, dt, a->m, a->n, dpre_s};
+  c.x[1] = {a->dup, dt, a->m, a->n, dpre_s};
+  c.y[0] = {a->w_gate, dt, a->n, a->k, w_s};
+  c.y[1] = {a->w_up, dt, a->n, a->k, w_s};
+  c.y[2] = {a->x, dt, a->m, a->k, x_s};
+  c.d[0] = {a->dx, dt, a->m, a->k, dx_s};
+  c.d[1] = {a->dw_gate, dt, a->n, a->k, dw_s};
+  c.d[2] = {a->dw_up, dt, a->n, a->k, dw_s};
+  c.p.rows = a->m; c.p.cols = a->k; c.p.reduce = a->n;
+  c.p.bf16 = dt == CFK_BF16; c.p.out = dt;
 
+  const ProductPlan plan = plan_backward(a);
+  if (too_many_tiles(plan.pair)) return CFK_ERR_UNSUPPORTED;
   const cudaError_t e = dt == CFK_FP16 ? launch_gate_grad<CFK_FP16>(a, dh_s, pre_s, dpre_s, st)
                                        : launch_gate_grad<CFK_BF16>(a, dh_s, pre_s, dpre_s, st);
   if (note_cuda(e, "gate gradient launch") != cudaSuccess) return CFK_ERR_LAUNCH;
   int rc = CFK_OK;
-  if (a->dx && (rc = run_product<kGradX>(gx, st))) return rc;
-  if (a->dw_gate) rc = run_product<kGradW>(gw, st);
-  return rc;
+  if (plan.few.tt > 0 && (rc = run_few<kGrad>(c, plan.few, st))) return rc;
+  return plan.pair.jobs > 0 ? run_pairs<kGrad>(c, plan.pair, st) : CFK_OK;
 }

@@ -1,0 +1,4 @@
+#include "ffn_few_sm100.cuh"
+namespace cfk {
+template int launch_few_product<kProductI8>(const ProductMaps&, const ProductParams&, const FewPlan&, cudaStream_t);
+}

@@ -1,4 +1,4 @@
-// Parameters and launchers of the feed-forward products (ffn.cu, ffn_pair_sm100.cuh).
+// Parameters, cuts and launchers of the feed-forward products (ffn.cu, ffn_pair_sm100.cuh, ffn_few_sm100.cuh).
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -11,15 +11,17 @@ enum ProductMode {
   kProductI8 = 0,   // C = scaled (A B^T), 8-bit integers
   kGated16 = 1,     // h = act(x Wg^T) * (x Wu^T), 16 bits
   kGatedI8 = 2,     // the same, 8-bit integers with scales
-  kGradX = 3,       // dx = dgate Wg + dup Wu: one reduction over the channels of both
-  kGradW = 4        // dw_gate = dgate^T x, dw_up = dup^T x: a batch of two products, reduced over the tokens
+  kGrad = 3         // dx = dgate Wg + dup Wu, one reduction over the channels of both; dw_gate = dgate^T x, dw_up = dup^T x, a batch
+                    // of two products reduced over the tokens
 };
 
+// Operands and results.  kProductI8, kGated*: x[0] tokens, y weights (w_gate, w_up), d result (h, gate, up).
+// kGrad: x dgate and dup, y w_gate, w_up and the tokens, d dx, dw_gate and dw_up.
+struct ProductMaps { CUtensorMap x[2], y[3], d[3]; };
+
 struct ProductParams {
-  int rows, cols;          // of the result (kGated*: of h)
-  int reduce;              // length of the reduction (kGradX: of each of its two parts)
-  int tiles_r, tiles_c;    // tiles of the result
-  int batches;             // 2 for kGradW
+  int rows, cols;          // of the result (kGrad: of dx)
+  int reduce;              // length of the reduction (kGrad: of each of the two parts of dx)
   int bf16;                // operands (16-bit modes)
   int out;                 // cfk_dtype of the results
   int act, keep;           // kGated*: activation; the pre-activations are written too
@@ -27,20 +29,38 @@ struct ProductParams {
   const float* col_scale;  // of the channels (kGatedI8: of w_gate)
   const float* col_scale2; // kGatedI8: of w_up
   const float* bias;       // kProductI8, or null
-  // A TMA store writes whole 16-byte pieces: behind the last element of a row it would put zeros up to the next multiple of 16 bytes.
-  // So the descriptors of the results end at the last whole piece, column `whole`, and the columns from there on are
-  // stored one by one.
-  int whole;
-  void* d[3];
+  void* d[3];              // results and the distance of their rows
   int64_t d_stride[3];
   int* status;
 };
 
-// Operands and results of a product.  x: tokens (kGradX: dgate, dup; kGradW: dgate, dup); y: weights (kGated*, kGradX: w_gate,
-// w_up; kGradW: x); d: the result (kGated*: h, gate, up; kGradW: dw_gate, dw_up).
-struct ProductMaps { CUtensorMap x[2], y[2], d[3]; };
+// One list of output tiles of the kernel on CTA pairs (256 rows x 2 bn accumulator columns each).
+struct PairJob {
+  int kind;                // kGrad: 0 dx, 1 dw_gate and dw_up
+  int rows, cols;          // of the result
+  int reduce;              // of a part of the reduction
+  int bn;                  // accumulator columns per CTA: 64, 96 or 128.  A tile has bn columns of h, 2 bn of any other result
+  int tiles_r, tiles_c, batches;
+};
+// The pairs take the tiles of the first list in turn.  Those that get one more of them than the others take `share` tiles of the second
+// list each, the others what is left.
+struct PairPlan { PairJob job[2]; int jobs, pairs, share; };
 
 template <int MODE>
-int launch_pair_product(const ProductMaps& maps, const ProductParams& p, cudaStream_t stream);
+int launch_pair_product(const ProductMaps& maps, const ProductParams& p, const PairPlan& plan, cudaStream_t stream);
+
+// How the kernel for few tokens cuts a product (kGrad: dx).
+struct FewPlan {
+  int tt;                  // tokens per tile; 0: the product runs on CTA pairs
+  int splits;              // CTAs of a cluster that share a tile's reduction, 1..8
+  int stages;              // of the ring
+  int tiles_ch, tiles_tok; // tiles of 128 channels x tt tokens
+};
+constexpr int kFewMaxStages = 12, kFewHead = 1024 + 256;                     // alignment slack and the barrier block
+constexpr int kFewSmemHalf = 113 * 1024, kFewSmemFull = 226 * 1024;          // bytes of a CTA: two per SM, one per SM
+constexpr int few_weights(int mode) { return mode == kGated16 || mode == kGatedI8 ? 2 : 1; }   // weights a tile reads per k-block
+
+template <int MODE>
+int launch_few_product(const ProductMaps& maps, const ProductParams& p, const FewPlan& f, cudaStream_t stream);
 
 }  // namespace cfk
