@@ -22,7 +22,8 @@ STATUS_NAMES = {0: "OK", 1: "INVALID_ARG", 2: "UNSUPPORTED", 3: "DESCRIPTOR", 4:
 
 EXPORTS = ["cfk_fmha_forward", "cfk_fmha_forward_static", "cfk_gemm", "cfk_fill", "cfk_convert", "cfk_device_status",
            "cfk_last_cuda_error", "cfk_version", "cfk_selftest_umma", "cfk_umma_peak", "cfk_selftest_wait_gives_up", "cfk_selftest_wait_gives_up_static", "cfk_set_tunable", "cfk_get_tunable", "cfk_fmha_plan", "cfk_gemm_plan",
-           "cfk_quantize_rows", "cfk_gemm_i8", "cfk_ffn_gated", "cfk_ffn_gated_backward"]
+           "cfk_quantize_rows", "cfk_gemm_i8", "cfk_ffn_gated", "cfk_ffn_gated_backward",
+           "cfk_gemm_i8_plan", "cfk_ffn_gated_plan", "cfk_ffn_gated_backward_plan"]
 
 TUNE_FMHA_EXP_EMU, TUNE_FMHA_GROUP_MB, TUNE_FMHA_KERNEL, TUNE_FMHA_GRID, TUNE_FMHA_SCHED = 0, 1, 2, 3, 4
 
@@ -127,6 +128,9 @@ class CfkLib:
         L.cfk_gemm_i8.argtypes = [C.POINTER(GemmI8Args), C.c_void_p]
         L.cfk_ffn_gated.argtypes = [C.POINTER(FfnGatedArgs), C.c_void_p]
         L.cfk_ffn_gated_backward.argtypes = [C.POINTER(FfnGatedBackwardArgs), C.c_void_p]
+        L.cfk_gemm_i8_plan.argtypes = [C.POINTER(GemmI8Args), C.POINTER(C.c_int)]
+        L.cfk_ffn_gated_plan.argtypes = [C.POINTER(FfnGatedArgs), C.POINTER(C.c_int)]
+        L.cfk_ffn_gated_backward_plan.argtypes = [C.POINTER(FfnGatedBackwardArgs), C.POINTER(C.c_int)]
         L.cfk_device_status.argtypes = [C.POINTER(C.c_int)]
         L.cfk_last_cuda_error.restype = C.c_char_p
         L.cfk_selftest_umma.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p] + [C.c_int] * 5 + [C.c_void_p]
@@ -212,6 +216,17 @@ class CfkLib:
                                  pre_stride, dpre_stride, dx_stride, dw_stride), stream)
         if rc:
             raise CfkError(rc, self.last_error())
+
+    def ffn_plan(self, args):
+        """(few-token kernel, tile width, parts of the reduction) of a GemmI8Args or FfnGatedArgs call; of FfnGatedBackwardArgs those
+        of dx and the tile width of the weights' gradients.  Launches nothing, needs no device."""
+        call, n = {GemmI8Args: (self.lib.cfk_gemm_i8_plan, 3), FfnGatedArgs: (self.lib.cfk_ffn_gated_plan, 3),
+                   FfnGatedBackwardArgs: (self.lib.cfk_ffn_gated_backward_plan, 4)}[type(args)]
+        plan = (C.c_int * n)()
+        rc = int(call(C.byref(args), plan))
+        if rc:
+            raise CfkError(rc, self.last_error())
+        return tuple(plan)
 
     def fmha_plan(self, args: FmhaArgs):
         """(kernel, key parts, remainder rows, key parts of the remainder) of a call; launches nothing, needs no device."""

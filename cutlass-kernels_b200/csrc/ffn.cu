@@ -12,6 +12,8 @@
 
 namespace cfk {
 
+static int64_t packed(int64_t stride, int cols) { return stride == 0 ? cols : stride; }
+
 // dgate = dh * up * act'(gate), dup = dh * act(gate).  Memory bound: three 16-bit values in, two out, 16 bytes per access, a thread
 // reads its elements of all three before it writes, so the results may take the place of gate and up.
 template <int DT, int ACT>
@@ -64,8 +66,8 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const uint16_t* dh, cons
 }
 
 template <int DT>
-static cudaError_t launch_gate_grad(const cfk_ffn_gated_backward_args* a, int64_t dh_s, int64_t pre_s, int64_t dpre_s,
-                                    cudaStream_t st) {
+static cudaError_t launch_gate_grad(const cfk_ffn_gated_backward_args* a, cudaStream_t st) {
+  const int64_t dh_s = packed(a->dh_stride, a->n), pre_s = packed(a->pre_stride, a->n), dpre_s = packed(a->dpre_stride, a->n);
   const uint32_t nvec = (uint32_t)((a->n + 7) / 8), total = (uint32_t)a->m * nvec;
   auto kern = a->activation == CFK_ACT_SILU ? gate_grad_kernel<DT, CFK_ACT_SILU>
               : a->activation == CFK_ACT_GELU ? gate_grad_kernel<DT, CFK_ACT_GELU>
@@ -106,7 +108,7 @@ static float plan_few(int mode, int rows, int cols, int reduce, FewPlan* best) {
     const long long tiles = (long long)tiles_ch * tiles_tok;
     if (tiles > 65536) continue;
     const float l2 = (float)tiles * (float)nkb * (float)stage / 13.5e6f;
-    const float dram = (float)tiles_ch * (float)nkb * (float)(nw * 16384) / 5.2e6f;
+    const float dram = (float)tiles_ch * (float)nkb * (float)(nw * 16384) / 5.6e6f;
     for (int i = 0; i < 6; ++i) {
       const int s = kSplits[i];
       if (s > nkb) break;
@@ -145,14 +147,15 @@ static float plan_pairs(int mode, PairPlan* plan) {
   for (int w = 0; w < (plan->jobs > 1 ? 9 : 3); ++w) {
     const int width[2] = {w % 3, w / 3};
     long long tiles[2] = {0, 0};
-    float each[2] = {0.f, 0.f}, last[2] = {0.f, 0.f}, bytes = 0.f;
+    float each[2] = {0.f, 0.f}, last[2] = {0.f, 0.f}, l2 = 0.f, dram = 0.f;      // last two: bytes
     for (int i = 0; i < plan->jobs; ++i) {
       PairJob& j = plan->job[i];
       const int bn = kWidth[width[i]], nkb = k_blocks(mode, j.reduce) * (mode == kGrad && j.kind == 0 ? 2 : 1);
       tiles[i] = set_width(&j, gated, bn);
       last[i] = 1.15f * (float)bn / 128.f;
       each[i] = 1.5f + fmaxf((float)nkb * kBlock[mode == kGrad][width[i]], last[i]);
-      bytes += (float)tiles[i] * (float)nkb * (float)(32768 + 2 * bn * 128);
+      l2 += (float)tiles[i] * (float)nkb * (float)(32768 + 2 * bn * 128);
+      dram += (float)nkb * 128.f * ((float)j.tiles_r * 256.f + (float)j.tiles_c * (float)(2 * bn)) * (float)j.batches;
     }
     const long long all = tiles[0] + tiles[1], pairs = all < kPairs ? all : kPairs;
     const long long most = tiles[0] / pairs, more = tiles[0] % pairs;      // `more` pairs have most + 1 tiles of the first list
@@ -170,7 +173,7 @@ static float plan_pairs(int mode, PairPlan* plan) {
         if (longest == 0.f || fmaxf(a, b) < longest) { longest = fmaxf(a, b); share = s; }
       }
     }
-    const float t = 2.5f + fmaxf(longest, bytes / 12.5e6f);
+    const float t = 2.5f + fmaxf(longest, fmaxf(l2 / 12.5e6f, dram / 4.2e6f));
     if (best_t == 0.f || t < best_t) {
       best_t = t;
       best = *plan;
@@ -235,16 +238,17 @@ struct Matrix {
   int dtype, rows, cols;
   int64_t stride;
 };
-// Read or written in boxes of `box_bytes` (which is the swizzle too) x `box_rows` rows.
-static int encode(CUtensorMap* map, const Matrix& m, int box_rows, int box_bytes = 128) {
+static bool rows_ok(const Matrix& m) { return rows_ok(m.base, m.dtype, m.cols, m.stride); }
+// Read in boxes of 128 bytes x `box_rows` rows.
+static int encode(CUtensorMap* map, const Matrix& m, int box_rows) {
   const uint64_t esz = (uint64_t)dtype_size(m.dtype);
   const uint64_t dims[3] = {(uint64_t)m.cols, (uint64_t)m.rows, 1};
   const uint64_t strides[2] = {(uint64_t)m.stride * esz, (uint64_t)m.stride * esz};
-  const uint32_t box[3] = {(uint32_t)(box_bytes / esz), (uint32_t)box_rows, 1};
-  return encode_tiled(map, m.dtype, 3, m.base, dims, strides, box, box_bytes);
+  const uint32_t box[3] = {(uint32_t)(128 / esz), (uint32_t)box_rows, 1};
+  return encode_tiled(map, m.dtype, 3, m.base, dims, strides, box, 128);
 }
 
-// Operands and results as in ProductMaps; unused ones have a null base.
+// Operands and results as in ProductMaps and ProductParams; unused ones have a null base.
 struct ProductCall {
   Matrix x[2], y[3], d[3];
   ProductParams p;
@@ -253,9 +257,11 @@ struct ProductCall {
 static int prepare_results(const ProductCall& c, ProductParams* p) {
   int rc = CFK_OK;
   p->status = device_status_block(&rc);
+  p->wide = 1;
   for (int i = 0; i < 3; ++i) {
     p->d[i] = const_cast<void*>(c.d[i].base);
     p->d_stride[i] = c.d[i].stride;
+    if (((uintptr_t)p->d[i] | (uintptr_t)(c.d[i].stride * dtype_size(c.d[i].dtype))) & 31u) p->wide = 0;
   }
   return rc;
 }
@@ -281,12 +287,8 @@ static int run_pairs(const ProductCall& c, const PairPlan& plan, cudaStream_t st
   int rc = prepare_results(c, &p);
   for (int i = 0; i < 2 && rc == CFK_OK; ++i)
     if (c.x[i].base) rc = encode(&maps.x[i], c.x[i], MODE == kGrad ? 64 : 128);
-  for (int i = 0; i < 3 && rc == CFK_OK; ++i) {
+  for (int i = 0; i < 3 && rc == CFK_OK; ++i)
     if (c.y[i].base) rc = encode(&maps.y[i], c.y[i], MODE == kGrad ? 64 : plan.job[0].bn);
-    Matrix d = c.d[i];         // up to the last whole 16 bytes of a row (ffn_pair_sm100.cuh, store_rest)
-    d.cols &= ~(16 / dtype_size(d.dtype) - 1);
-    if (rc == CFK_OK && d.base && d.cols > 0) rc = encode(&maps.d[i], d, 128, 32 * dtype_size(d.dtype));
-  }
   return rc ? rc : launch_pair_product<MODE>(maps, p, plan, stream);
 }
 
@@ -297,37 +299,30 @@ static int run_product(const ProductCall& c, cudaStream_t stream) {
   return too_many_tiles(plan.pair) ? CFK_ERR_UNSUPPORTED : run_pairs<MODE>(c, plan.pair, stream);
 }
 
-static int64_t packed(int64_t stride, int cols) { return stride == 0 ? cols : stride; }
 static bool is16(int dt) { return dt == CFK_FP16 || dt == CFK_BF16; }
 static bool floats_ok(const float* p) { return p != nullptr && ((uintptr_t)p & 3u) == 0; }
 
 // 32-bit sums of 8-bit products: k * 128 * 128 stays below 2^31
 constexpr int kMaxI8Reduction = 131071;
 
-}  // namespace cfk
-
-using namespace cfk;
-
-extern "C" int cfk_gemm_i8(const cfk_gemm_i8_args* a, cfk_stream_t stream) {
+// Argument checks of the three calls; what passes is ready to be cut and run.
+static int check_gemm_i8(const cfk_gemm_i8_args* a, ProductCall* c) {
   if (!a || !a->a || !a->b || !a->c || a->m <= 0 || a->n <= 0 || a->k <= 0) return CFK_ERR_INVALID_ARG;
   if (!is16(a->out_dtype) && a->out_dtype != CFK_FP32) return CFK_ERR_INVALID_ARG;
   if (!floats_ok(a->a_scale) || !floats_ok(a->b_scale) || ((uintptr_t)a->bias & 3u)) return CFK_ERR_INVALID_ARG;
-  ProductCall c;
-  std::memset(&c, 0, sizeof(c));
-  c.x[0] = {a->a, CFK_INT8, a->m, a->k, packed(a->a_stride, a->k)};
-  c.y[0] = {a->b, CFK_INT8, a->n, a->k, packed(a->b_stride, a->k)};
-  c.d[0] = {a->c, a->out_dtype, a->m, a->n, packed(a->c_stride, a->n)};
-  if (!rows_ok(a->a, CFK_INT8, a->k, c.x[0].stride) || !rows_ok(a->b, CFK_INT8, a->k, c.y[0].stride) ||
-      !rows_ok(a->c, a->out_dtype, a->n, c.d[0].stride))
-    return CFK_ERR_INVALID_ARG;
+  std::memset(c, 0, sizeof(*c));
+  c->x[0] = {a->a, CFK_INT8, a->m, a->k, packed(a->a_stride, a->k)};
+  c->y[0] = {a->b, CFK_INT8, a->n, a->k, packed(a->b_stride, a->k)};
+  c->d[0] = {a->c, a->out_dtype, a->m, a->n, packed(a->c_stride, a->n)};
+  if (!rows_ok(c->x[0]) || !rows_ok(c->y[0]) || !rows_ok(c->d[0])) return CFK_ERR_INVALID_ARG;
   if (a->k > kMaxI8Reduction) return CFK_ERR_UNSUPPORTED;
-  c.p.rows = a->m; c.p.cols = a->n; c.p.reduce = a->k;
-  c.p.out = a->out_dtype;
-  c.p.row_scale = a->a_scale; c.p.col_scale = a->b_scale; c.p.bias = a->bias;
-  return run_product<kProductI8>(c, (cudaStream_t)stream);
+  c->p.rows = a->m; c->p.cols = a->n; c->p.reduce = a->k;
+  c->p.out = a->out_dtype;
+  c->p.row_scale = a->a_scale; c->p.col_scale = a->b_scale; c->p.bias = a->bias;
+  return CFK_OK;
 }
 
-extern "C" int cfk_ffn_gated(const cfk_ffn_gated_args* a, cfk_stream_t stream) {
+static int check_gated(const cfk_ffn_gated_args* a, ProductCall* c) {
   if (!a || !a->x || !a->w_gate || !a->w_up || !a->h || a->m <= 0 || a->n <= 0 || a->k <= 0) return CFK_ERR_INVALID_ARG;
   const bool i8 = a->dtype == CFK_INT8;
   if ((!is16(a->dtype) && !i8) || !is16(a->out_dtype) || (!i8 && a->out_dtype != a->dtype)) return CFK_ERR_INVALID_ARG;
@@ -336,70 +331,110 @@ extern "C" int cfk_ffn_gated(const cfk_ffn_gated_args* a, cfk_stream_t stream) {
   if (i8 ? !floats_ok(a->x_scale) || !floats_ok(a->gate_scale) || !floats_ok(a->up_scale)
          : a->x_scale || a->gate_scale || a->up_scale)
     return CFK_ERR_INVALID_ARG;
-  ProductCall c;
-  std::memset(&c, 0, sizeof(c));
+  std::memset(c, 0, sizeof(*c));
   const int64_t w_stride = packed(a->w_stride, a->k), pre_stride = packed(a->pre_stride, a->n);
-  c.x[0] = {a->x, a->dtype, a->m, a->k, packed(a->x_stride, a->k)};
-  c.y[0] = {a->w_gate, a->dtype, a->n, a->k, w_stride};
-  c.y[1] = {a->w_up, a->dtype, a->n, a->k, w_stride};
-  c.d[0] = {a->h, a->out_dtype, a->m, a->n, packed(a->h_stride, a->n)};
+  c->x[0] = {a->x, a->dtype, a->m, a->k, packed(a->x_stride, a->k)};
+  c->y[0] = {a->w_gate, a->dtype, a->n, a->k, w_stride};
+  c->y[1] = {a->w_up, a->dtype, a->n, a->k, w_stride};
+  c->d[0] = {a->h, a->out_dtype, a->m, a->n, packed(a->h_stride, a->n)};
   if (a->gate) {
-    c.d[1] = {a->gate, a->out_dtype, a->m, a->n, pre_stride};
-    c.d[2] = {a->up, a->out_dtype, a->m, a->n, pre_stride};
+    c->d[1] = {a->gate, a->out_dtype, a->m, a->n, pre_stride};
+    c->d[2] = {a->up, a->out_dtype, a->m, a->n, pre_stride};
+    if (!rows_ok(c->d[1]) || !rows_ok(c->d[2])) return CFK_ERR_INVALID_ARG;
+    if (a->gate == a->up || a->gate == a->h || a->up == a->h) return CFK_ERR_INVALID_ARG;
   }
-  if (!rows_ok(a->x, a->dtype, a->k, c.x[0].stride) || !rows_ok(a->w_gate, a->dtype, a->k, w_stride) ||
-      !rows_ok(a->w_up, a->dtype, a->k, w_stride) || !rows_ok(a->h, a->out_dtype, a->n, c.d[0].stride))
-    return CFK_ERR_INVALID_ARG;
-  if (a->gate && (!rows_ok(a->gate, a->out_dtype, a->n, pre_stride) || !rows_ok(a->up, a->out_dtype, a->n, pre_stride)))
-    return CFK_ERR_INVALID_ARG;
+  if (!rows_ok(c->x[0]) || !rows_ok(c->y[0]) || !rows_ok(c->y[1]) || !rows_ok(c->d[0])) return CFK_ERR_INVALID_ARG;
   if (i8 && a->k > kMaxI8Reduction) return CFK_ERR_UNSUPPORTED;
-  c.p.rows = a->m; c.p.cols = a->n; c.p.reduce = a->k;
-  c.p.bf16 = a->dtype == CFK_BF16; c.p.out = a->out_dtype;
-  c.p.act = a->activation; c.p.keep = a->gate != nullptr;
-  c.p.row_scale = a->x_scale; c.p.col_scale = a->gate_scale; c.p.col_scale2 = a->up_scale;
-  return i8 ? run_product<kGatedI8>(c, (cudaStream_t)stream) : run_product<kGated16>(c, (cudaStream_t)stream);
+  c->p.rows = a->m; c->p.cols = a->n; c->p.reduce = a->k;
+  c->p.bf16 = a->dtype == CFK_BF16; c->p.out = a->out_dtype;
+  c->p.act = a->activation; c->p.keep = a->gate != nullptr;
+  c->p.row_scale = a->x_scale; c->p.col_scale = a->gate_scale; c->p.col_scale2 = a->up_scale;
+  return CFK_OK;
 }
 
-extern "C" int cfk_ffn_gated_backward(const cfk_ffn_gated_backward_args* a, cfk_stream_t stream) {
+static int check_backward(const cfk_ffn_gated_backward_args* a, ProductCall* c) {
   if (!a || !a->dh || !a->x || !a->w_gate || !a->w_up || !a->gate || !a->up || !a->dgate || !a->dup) return CFK_ERR_INVALID_ARG;
   if (a->m <= 0 || a->n <= 0 || a->k <= 0 || !is16(a->dtype)) return CFK_ERR_INVALID_ARG;
   if (a->activation < CFK_ACT_SILU || a->activation > CFK_ACT_RELU) return CFK_ERR_INVALID_ARG;
   if ((a->dw_gate == nullptr) != (a->dw_up == nullptr)) return CFK_ERR_INVALID_ARG;
   const int dt = a->dtype;
-  const int64_t dh_s = packed(a->dh_stride, a->n), x_s = packed(a->x_stride, a->k), w_s = packed(a->w_stride, a->k);
   const int64_t pre_s = packed(a->pre_stride, a->n), dpre_s = packed(a->dpre_stride, a->n);
-  const int64_t dx_s = packed(a->dx_stride, a->k), dw_s = packed(a->dw_stride, a->k);
-  if (!rows_ok(a->dh, dt, a->n, dh_s) || !rows_ok(a->x, dt, a->k, x_s) || !rows_ok(a->w_gate, dt, a->k, w_s) ||
-      !rows_ok(a->w_up, dt, a->k, w_s) || !rows_ok(a->gate, dt, a->n, pre_s) || !rows_ok(a->up, dt, a->n, pre_s) ||
-      !rows_ok(a->dgate, dt, a->n, dpre_s) || !rows_ok(a->dup, dt, a->n, dpre_s))
-    return CFK_ERR_INVALID_ARG;
-  if (a->dx && !rows_ok(a->dx, dt, a->k, dx_s)) return CFK_ERR_INVALID_ARG;
-  if (a->dw_gate && (!rows_ok(a->dw_gate, dt, a->k, dw_s) || !rows_ok(a->dw_up, dt, a->k, dw_s))) return CFK_ERR_INVALID_ARG;
+  const int64_t w_s = packed(a->w_stride, a->k), dw_s = packed(a->dw_stride, a->k);
+  std::memset(c, 0, sizeof(*c));
+  c->x[0] = {a->dgate, dt, a->m, a->n, dpre_s};
+  c->x[1] = {a->dup, dt, a->m, a->n, dpre_s};
+  c->y[0] = {a->w_gate, dt, a->n, a->k, w_s};
+  c->y[1] = {a->w_up, dt, a->n, a->k, w_s};
+  c->y[2] = {a->x, dt, a->m, a->k, packed(a->x_stride, a->k)};
+  c->d[0] = {a->dx, dt, a->m, a->k, packed(a->dx_stride, a->k)};
+  c->d[1] = {a->dw_gate, dt, a->n, a->k, dw_s};
+  c->d[2] = {a->dw_up, dt, a->n, a->k, dw_s};
+  const Matrix in[3] = {{a->dh, dt, a->m, a->n, packed(a->dh_stride, a->n)}, {a->gate, dt, a->m, a->n, pre_s},
+                        {a->up, dt, a->m, a->n, pre_s}};
+  for (int i = 0; i < 3; ++i)
+    if (!rows_ok(in[i]) || !rows_ok(c->y[i]) || (i < 2 && !rows_ok(c->x[i])) || (c->d[i].base && !rows_ok(c->d[i])))
+      return CFK_ERR_INVALID_ARG;
   // the only buffers that may be shared: dgate on gate, dup on up, row for row
   if (a->dgate == a->dup || a->dgate == a->up || a->dup == a->gate || a->dgate == a->dh || a->dup == a->dh) return CFK_ERR_INVALID_ARG;
   if ((a->dgate == a->gate || a->dup == a->up) && pre_s != dpre_s) return CFK_ERR_INVALID_ARG;
   if ((long long)a->m * ((a->n + 7) / 8) > 0xffffff00LL) return CFK_ERR_UNSUPPORTED;
-  const cudaStream_t st = (cudaStream_t)stream;
+  c->p.rows = a->m; c->p.cols = a->k; c->p.reduce = a->n;
+  c->p.bf16 = dt == CFK_BF16; c->p.out = dt;
+  return CFK_OK;
+}
 
+static int tell_plan(int rc, int mode, const ProductCall& c, int plan[3]) {
+  if (rc != CFK_OK || !plan) return rc != CFK_OK ? rc : CFK_ERR_INVALID_ARG;
+  const ProductPlan p = plan_product(mode, c.p.rows, c.p.cols, c.p.reduce);
+  plan[0] = p.few.tt > 0; plan[1] = p.few.tt > 0 ? p.few.tt : p.pair.job[0].bn; plan[2] = p.few.tt > 0 ? p.few.splits : 1;
+  return CFK_OK;
+}
+
+}  // namespace cfk
+
+using namespace cfk;
+
+extern "C" int cfk_gemm_i8(const cfk_gemm_i8_args* a, cfk_stream_t stream) {
   ProductCall c;
-  std::memset(&c, 0, sizeof(c));
-  c.x[0] = {a->dgate, dt, a->m, a->n, dpre_s};
-  c.x[1] = {a->dup, dt, a->m, a->n, dpre_s};
-  c.y[0] = {a->w_gate, dt, a->n, a->k, w_s};
-  c.y[1] = {a->w_up, dt, a->n, a->k, w_s};
-  c.y[2] = {a->x, dt, a->m, a->k, x_s};
-  c.d[0] = {a->dx, dt, a->m, a->k, dx_s};
-  c.d[1] = {a->dw_gate, dt, a->n, a->k, dw_s};
-  c.d[2] = {a->dw_up, dt, a->n, a->k, dw_s};
-  c.p.rows = a->m; c.p.cols = a->k; c.p.reduce = a->n;
-  c.p.bf16 = dt == CFK_BF16; c.p.out = dt;
+  const int rc = check_gemm_i8(a, &c);
+  return rc ? rc : run_product<kProductI8>(c, (cudaStream_t)stream);
+}
+extern "C" int cfk_gemm_i8_plan(const cfk_gemm_i8_args* a, int plan[3]) {
+  ProductCall c;
+  const int rc = check_gemm_i8(a, &c);
+  return tell_plan(rc, kProductI8, c, plan);
+}
 
+extern "C" int cfk_ffn_gated(const cfk_ffn_gated_args* a, cfk_stream_t stream) {
+  ProductCall c;
+  const int rc = check_gated(a, &c);
+  if (rc) return rc;
+  return a->dtype == CFK_INT8 ? run_product<kGatedI8>(c, (cudaStream_t)stream) : run_product<kGated16>(c, (cudaStream_t)stream);
+}
+extern "C" int cfk_ffn_gated_plan(const cfk_ffn_gated_args* a, int plan[3]) {
+  ProductCall c;
+  const int rc = check_gated(a, &c);
+  return tell_plan(rc, rc == CFK_OK && a->dtype == CFK_INT8 ? kGatedI8 : kGated16, c, plan);
+}
+
+extern "C" int cfk_ffn_gated_backward(const cfk_ffn_gated_backward_args* a, cfk_stream_t stream) {
+  ProductCall c;
+  int rc = check_backward(a, &c);
+  if (rc) return rc;
   const ProductPlan plan = plan_backward(a);
   if (too_many_tiles(plan.pair)) return CFK_ERR_UNSUPPORTED;
-  const cudaError_t e = dt == CFK_FP16 ? launch_gate_grad<CFK_FP16>(a, dh_s, pre_s, dpre_s, st)
-                                       : launch_gate_grad<CFK_BF16>(a, dh_s, pre_s, dpre_s, st);
+  const cudaStream_t st = (cudaStream_t)stream;
+  const cudaError_t e = a->dtype == CFK_FP16 ? launch_gate_grad<CFK_FP16>(a, st) : launch_gate_grad<CFK_BF16>(a, st);
   if (note_cuda(e, "gate gradient launch") != cudaSuccess) return CFK_ERR_LAUNCH;
-  int rc = CFK_OK;
   if (plan.few.tt > 0 && (rc = run_few<kGrad>(c, plan.few, st))) return rc;
   return plan.pair.jobs > 0 ? run_pairs<kGrad>(c, plan.pair, st) : CFK_OK;
+}
+extern "C" int cfk_ffn_gated_backward_plan(const cfk_ffn_gated_backward_args* a, int plan[4]) {
+  ProductCall c;
+  const int rc = check_backward(a, &c);
+  if (rc != CFK_OK || !plan) return rc != CFK_OK ? rc : CFK_ERR_INVALID_ARG;
+  const ProductPlan p = plan_backward(a);
+  plan[0] = p.few.tt > 0; plan[1] = p.few.tt; plan[2] = p.few.tt > 0 ? p.few.splits : 1; plan[3] = 0;
+  for (int i = 0; i < p.pair.jobs; ++i) plan[p.pair.job[i].kind == 0 ? 1 : 3] = p.pair.job[i].bn;
+  return CFK_OK;
 }

@@ -191,9 +191,9 @@ few_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_consta
   if (epilogue) {
     if constexpr (I8) {
       if (ch < p.cols) {
-        cs = __ldg(p.col_scale + ch);
-        if constexpr (GATED) cs2 = __ldg(p.col_scale2 + ch);
-        else if (p.bias != nullptr) bias = __ldg(p.bias + ch);
+        cs = p.col_scale[ch];
+        if constexpr (GATED) cs2 = p.col_scale2[ch];
+        else if (p.bias != nullptr) bias = p.bias[ch];
       }
     }
     done = mbar_wait_warp(bar_acc, 0, actx, kErrFewAcc);
@@ -205,7 +205,7 @@ few_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_consta
     const int token = tok0 + t0;
     float v[8], u[8];
     if constexpr (I8) {
-      const float rs = lane < n ? __ldg(p.row_scale + token + lane) : 0.f;     // n <= 8
+      const float rs = lane < n ? p.row_scale[token + lane] : 0.f;     // n <= 8
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float rsi = __shfl_sync(0xffffffffu, rs, i);

@@ -10,9 +10,10 @@
 //                is the column of dx: they are MN-major operands.  dw_gate, dw_up: a reduction over the tokens, along which neither
 //                operand is contiguous: both are MN-major.
 //
-// Roles, ring, tensor-memory double buffer and store path are those of gemm_kernel: warp 0 TMA, warp 1 of the leader
-// UMMA (cta_group::2), but two groups of four epilogue warps (with one, a tile's epilogue of 3 us was most of a short call) that store
-// with TMA, which clips at the result's edges.
+// Roles, ring and tensor-memory double buffer are those of gemm_kernel: warp 0 TMA, warp 1 of the leader UMMA (cta_group::2); but
+// two groups of four epilogue warps, which write whole sectors from registers.  (A TMA store writes whole 16-byte pieces, so behind
+// the last element of a row it would put zeros up to the next multiple of 16 bytes; and the hand-over of its staging tiles took 0.6 us
+// per 32 columns, most of a tile whose reduction is short.)
 // An MN-major operand lands as spans of 64 columns, [span][64 k-rows][128 bytes], each with the 128-byte swizzle; what lies
 // behind a matrix is zero-filled in both operands, so ragged reductions need no mask.
 //
@@ -28,61 +29,64 @@
 
 namespace cfk {
 
-constexpr int kErrPairFull = 211, kErrPairEmpty = 212, kErrPairAccFull = 213, kErrPairAccEmpty = 214, kErrPairStaged = 215,
-              kErrPairStageFree = 216;
+constexpr int kErrPairFull = 211, kErrPairEmpty = 212, kErrPairAccFull = 213, kErrPairAccEmpty = 214;
 
 struct PairCfg {
   static constexpr int TM = 256, TN = 256, BM = 128, BN = 128;     // tile of the pair; rows of X and of Y per CTA
   static constexpr int XB = BM * 128, YB = BN * 128;               // bytes per k-block
-  static constexpr int NSTAGE = 6;
+  static constexpr int NSTAGE = 7;
   static constexpr int GROUPS = 2;                                 // of four epilogue warps
-  static constexpr int STAGEB = 128 * 128;                         // staging per group: 128 rows x 32 columns of fp32, or twice 16 bits
-  static constexpr int SMEM_BYTES = 1024 + NSTAGE * (XB + YB) + GROUPS * STAGEB + 256;
+  static constexpr int SMEM_BYTES = 1024 + NSTAGE * (XB + YB) + 256;
   static constexpr int NTHREADS = 64 + GROUPS * 128;
-  static_assert(8 * (2 * NSTAGE + 4 + 4 * GROUPS) + 8 <= 256, "barrier block overflows");
+  static_assert(8 * (2 * NSTAGE + 4) + 8 <= 256, "barrier block overflows");
 };
 
-// 32 columns of 128 rows as a TMA store takes them: rows of 64 bytes with the 64-byte swizzle (16-byte piece index XOR bits 1-2 of
-// the row), or of 128 bytes with the 128-byte swizzle (XOR bits 0-2) for fp32.
-__device__ __forceinline__ uint32_t staged_at(uint32_t tile, int r, uint32_t byte, bool out32) {
-  return out32 ? tile + r * 128 + (((byte >> 4) ^ (uint32_t)(r & 7)) << 4) + (byte & 15u)
-               : tile + r * 64 + (((byte >> 4) ^ (uint32_t)((r >> 1) & 3)) << 4) + (byte & 15u);
+// 32 columns of a row, from `col` on, as far as they exist.  A thread writes whole 32-byte sectors where rows start at multiples of
+// 32 bytes (`wide`), and nothing behind the row's end.
+__device__ __forceinline__ void st_global_32(void* to, const uint32_t (&w)[32], int at) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[at]), "r"(w[at + 1]), "r"(w[at + 2]),
+               "r"(w[at + 3]), "r"(w[at + 4]), "r"(w[at + 5]), "r"(w[at + 6]), "r"(w[at + 7]) : "memory");
 }
-__device__ __forceinline__ void stage_row16(uint32_t tile, int r, bool bf16, const float (&v)[32]) {
+__device__ __forceinline__ void store_columns(const ProductParams& p, int which, int row, int col, int cols, const float (&v)[32]) {
+  const bool out32 = p.out == CFK_FP32, bf16 = p.out == CFK_BF16;
+  const int64_t at = row * p.d_stride[which] + col;
+  const int n = cols - col;                      // columns that exist, if fewer than 32
+  uint32_t w[32];
+  if (out32) {
+    float* d = reinterpret_cast<float*>(p.d[which]) + at;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const uint32_t w0 = pack_out(bf16, v[g * 8], v[g * 8 + 1]), w1 = pack_out(bf16, v[g * 8 + 2], v[g * 8 + 3]);
-    const uint32_t w2 = pack_out(bf16, v[g * 8 + 4], v[g * 8 + 5]), w3 = pack_out(bf16, v[g * 8 + 6], v[g * 8 + 7]);
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staged_at(tile, r, g * 16, false)), "r"(w0), "r"(w1), "r"(w2),
-                 "r"(w3) : "memory");
-  }
-}
-__device__ __forceinline__ void stage_row32(uint32_t tile, int r, const float (&v)[32]) {
+    for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
+    if (n >= 32 && p.wide) {
 #pragma unroll
-  for (int g = 0; g < 8; ++g)
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staged_at(tile, r, g * 16, true)),
-                 "r"(__float_as_uint(v[g * 4])), "r"(__float_as_uint(v[g * 4 + 1])), "r"(__float_as_uint(v[g * 4 + 2])),
-                 "r"(__float_as_uint(v[g * 4 + 3])) : "memory");
-}
-
-// A TMA store writes whole 16-byte pieces: behind the last element of a row it would put zeros up to the next multiple of 16
-// bytes.  So the descriptors of the results end at the last whole piece, column `whole`, and the columns from there on are
-// stored one by one, read back from this thread's own row of the staged 32 columns that begin at `col`.
-__device__ __forceinline__ int whole_columns(int cols, bool out32) { return cols & ~(out32 ? 3 : 7); }
-__device__ __forceinline__ void store_rest(const ProductParams& p, int which, bool out32, uint32_t tile, int r, int row, int col,
-                                           int whole, int cols) {
-  const int end = cols < col + 32 ? cols : col + 32;
-  for (int c = whole > col ? whole : col; c < end; ++c) {
-    const uint32_t from = staged_at(tile, r, (uint32_t)((c - col) * (out32 ? 4 : 2)), out32);
-    const int64_t at = row * p.d_stride[which] + c;
-    if (out32) {
-      uint32_t v;
-      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
-      reinterpret_cast<uint32_t*>(p.d[which])[at] = v;
+      for (int i = 0; i < 32; i += 8) st_global_32(d + i, w, i);
     } else {
-      uint16_t v;
-      asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
-      reinterpret_cast<uint16_t*>(p.d[which])[at] = v;
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        if (i + 4 <= n) *reinterpret_cast<uint4*>(d + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        else {
+#pragma unroll
+          for (int e = i; e < i + 4; ++e)
+            if (e < n) d[e] = v[e];
+        }
+      }
+    }
+  } else {
+    uint16_t* d = reinterpret_cast<uint16_t*>(p.d[which]) + at;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = pack_out(bf16, v[2 * i], v[2 * i + 1]);
+    if (n >= 32 && p.wide) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 8) st_global_32(d + 2 * i, w, i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) {
+        if (i + 8 <= n) *reinterpret_cast<uint4*>(d + i) = make_uint4(w[i / 2], w[i / 2 + 1], w[i / 2 + 2], w[i / 2 + 3]);
+        else {
+#pragma unroll
+          for (int e = i; e < i + 8; ++e)
+            if (e < n) d[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+        }
+      }
     }
   }
 }
@@ -139,16 +143,13 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
   const uint32_t sX = smem_base;
   const uint32_t sY = smem_base + C::NSTAGE * C::XB;
-  const uint32_t sStage = sY + C::NSTAGE * C::YB;            // [GROUPS] output staging
-  const uint32_t sBar = sStage + C::GROUPS * C::STAGEB;
+  const uint32_t sBar = sY + C::NSTAGE * C::YB;
   const uint32_t bar_full = sBar;                            // [NSTAGE] leader: both CTAs' loads of a stage landed
   const uint32_t bar_empty = sBar + 8 * C::NSTAGE;           // [NSTAGE] each CTA: its stage was consumed
   const uint32_t bar_acc_full = bar_empty + 8 * C::NSTAGE;   // [2] each CTA: accumulator complete
   const uint32_t bar_acc_empty = bar_acc_full + 16;          // [2] leader: all epilogue warps of both have read it
-  const uint32_t bar_staged = bar_acc_empty + 16;            // [GROUPS][2] a staging tile is complete (4 epilogue warps)
-  const uint32_t bar_stage_free = bar_staged + 16 * C::GROUPS;   // [GROUPS][2] the TMA store has read a staging tile
   uint8_t* gBar = smem_gen + (sBar - smem_base);
-  const uint32_t off_misc = 8 * (2 * C::NSTAGE + 4 + 4 * C::GROUPS);
+  const uint32_t off_misc = 8 * (2 * C::NSTAGE + 4);
   volatile uint32_t* s_tmem_base = reinterpret_cast<volatile uint32_t*>(gBar + off_misc);
   volatile uint32_t* s_abort = reinterpret_cast<volatile uint32_t*>(gBar + off_misc + 4);
   const AbortCtx actx{s_abort, p.status};
@@ -162,7 +163,6 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
   if (tid == 0) {
     for (int i = 0; i < C::NSTAGE; ++i) { mbar_init(bar_full + 8 * i, 2); mbar_init(bar_empty + 8 * i, 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(bar_acc_full + 8 * i, 1); mbar_init(bar_acc_empty + 8 * i, 2 * 4 * C::GROUPS); }
-    for (int i = 0; i < 2 * C::GROUPS; ++i) { mbar_init(bar_staged + 8 * i, 4); mbar_init(bar_stage_free + 8 * i, 1); }
     *s_abort = 0u;
     fence_barrier_init();
   }
@@ -253,125 +253,82 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
       }
     }
   } else {
-    // epilogue warps 2..9 in two groups of four; warp w may touch TMEM lanes 32*(w%4) .. +31.  A tile leaves in chunks of 32 columns,
-    // taken by the groups in turn, each through staging of the group's own (two tiles that alternate; one of fp32).  With `keep`
-    // the chunks of h, gate and up of the same columns follow each other.
+    // epilogue warps 2..9 in two groups of four, which take 32 columns of the tile in turn; warp w may touch TMEM lanes
+    // 32*(w%4) .. +31, a row per thread.
     const int grp = (warp - 2) >> 2;
     const int q = warp & 3;
     const int r = q * 32 + lane;                       // row within this CTA's 128 rows
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     const uint32_t leader_acc_empty = map_to_cta(bar_acc_empty, 0);
-    const uint32_t my_stage = sStage + grp * C::STAGEB, my_staged = bar_staged + 16 * grp, my_free = bar_stage_free + 16 * grp;
-    const bool out32 = MODE == kProductI8 && p.out == CFK_FP32, out_bf16 = p.out == CFK_BF16;
-    const int kinds = GATED && p.keep ? 3 : 1;         // chunks per 32 columns: h, gate, up
-    const bool storer = ((warp - 2) & 3) == 0 && lane == 0;
     int local = 0;
-    uint32_t n = 0;                                    // chunks this group has staged so far
     bool ok = true;
     for (PairTile t; ok && pair_tile(t, plan, pair_id, local, GRAD, KB); ++local) {
       const int buf = local & 1;
-      const int row0 = t.tr * C::TM + (int)rank * C::BM, row = row0 + r;
+      const int row = t.tr * C::TM + (int)rank * C::BM + r;
       const int tcols = GATED ? t.bn : 2 * t.bn, col0 = t.tc * tcols;
       const int end = t.cols - col0 < tcols ? t.cols - col0 : tcols;     // columns of the tile that exist
-      const int whole = whole_columns(t.cols, out32);
       const uint32_t acc = tmem_base + lane_base + buf * C::TN;
+      const bool inside = row < t.rows;
       float rs = 0.f;
-      if constexpr (I8) rs = row < t.rows ? __ldg(p.row_scale + row) : 0.f;
+      if constexpr (I8) rs = inside ? p.row_scale[row] : 0.f;
       ok = mbar_wait_warp(bar_acc_full + 8 * buf, (local >> 1) & 1, actx, kErrPairAccFull);
       if (!ok) break;
       tc_fence_after_sync();
-      const int nchunk = (end + 31) / 32 * kinds;
 #pragma unroll 1
-      for (int ch = grp; ch < nchunk; ch += C::GROUPS, ++n) {
-        const int kind = kinds == 1 ? 0 : ch % 3;
-        const int which = GRAD ? (t.kind == 0 ? 0 : 1 + t.batch) : kind;   // result
-        const int cb = (kinds == 1 ? ch : ch / 3) * 32;                    // first column of the chunk within the tile
-        const uint32_t sb = out32 ? 0u : n & 1u, use = out32 ? n : n >> 1; // staging tile and how often it was used before
-        const uint32_t stage = my_stage + sb * (C::STAGEB / 2);
-        if (use >= 1u) {   // the store that last used this staging tile has read it
-          ok = mbar_wait_warp(my_free + 8 * sb, (use & 1u) ^ 1u, actx, kErrPairStageFree);
-          if (!ok) break;
-        }
-        const int col = col0 + cb + lane;                      // this lane's column: its scales reach the others by shuffle
+      for (int cb = grp * 32; cb < end; cb += C::GROUPS * 32) {
+        const int col = col0 + cb, mine = col + lane;          // this lane's column: its scales reach the others by shuffle
         float v[32];
         if constexpr (GATED) {
-          float gs = 1.f, us = 1.f;
-          if constexpr (I8) {
-            gs = col < t.cols ? __ldg(p.col_scale + col) : 0.f;
-            us = col < t.cols ? __ldg(p.col_scale2 + col) : 0.f;
-          }
           float u[32];
-          uint32_t w[32];
-          if (kind != 2) {
-            tmem_ld_x32(acc + cb, w);
+          uint32_t w[32], x[32];
+          tmem_ld_x32(acc + cb, w);
+          tmem_ld_x32(acc + t.bn + cb, x);
+          if constexpr (I8) {
+            const float gs = mine < t.cols ? p.col_scale[mine] : 0.f;
+            const float us = mine < t.cols ? p.col_scale2[mine] : 0.f;
             tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              if constexpr (I8) v[i] = __int2float_rn((int)w[i]) * rs * __shfl_sync(0xffffffffu, gs, i);
-              else v[i] = __uint_as_float(w[i]);
+              v[i] = __int2float_rn((int)w[i]) * rs * __shfl_sync(0xffffffffu, gs, i);
+              u[i] = __int2float_rn((int)x[i]) * rs * __shfl_sync(0xffffffffu, us, i);
             }
-          }
-          if (kind != 1) {
-            tmem_ld_x32(acc + t.bn + cb, w);
+          } else {
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if constexpr (I8) u[i] = __int2float_rn((int)w[i]) * rs * __shfl_sync(0xffffffffu, us, i);
-              else u[i] = __uint_as_float(w[i]);
-            }
+            for (int i = 0; i < 32; ++i) { v[i] = __uint_as_float(w[i]); u[i] = __uint_as_float(x[i]); }
           }
-          if (kind == 0) gate_columns(p.act, v, u);
-          if (kind == 2) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = u[i];
+          if (p.keep && inside) {
+            store_columns(p, 1, row, col, t.cols, v);
+            store_columns(p, 2, row, col, t.cols, u);
           }
-          stage_row16(stage, r, out_bf16, v);
+          gate_columns(p.act, v, u);
+          if (inside) store_columns(p, 0, row, col, t.cols, v);
         } else {
           uint32_t w[32];
           tmem_ld_x32(acc + cb, w);
-          tmem_wait_ld();
           if constexpr (I8) {
-            const float cs = col < t.cols ? __ldg(p.col_scale + col) : 0.f;
-            const float bs = p.bias != nullptr && col < t.cols ? __ldg(p.bias + col) : 0.f;
+            const float cs = mine < t.cols ? p.col_scale[mine] : 0.f;
+            const float bs = p.bias != nullptr && mine < t.cols ? p.bias[mine] : 0.f;
+            tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = __int2float_rn((int)w[i]) * rs * __shfl_sync(0xffffffffu, cs, i);
             if (p.bias != nullptr) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, bs, i);
             }
-            if (out32) stage_row32(stage, r, v);
-            else stage_row16(stage, r, out_bf16, v);
           } else {
+            tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(w[i]);
-            stage_row16(stage, r, out_bf16, v);
           }
+          if (inside) store_columns(p, GRAD ? (t.kind == 0 ? 0 : 1 + t.batch) : 0, row, col, t.cols, v);
         }
-        if (row < t.rows && col0 + cb + 32 > whole) store_rest(p, which, out32, stage, r, row, col0 + cb, whole, t.cols);
-        fence_proxy_async_smem();
-        mbar_arrive_warp(my_staged + 8 * sb);
-        if (storer) {
-          if (!mbar_wait(my_staged + 8 * sb, use & 1u, actx, kErrPairStaged)) { ok = false; }
-          else {
-            if (col0 + cb < whole) tma_store_3d(&maps.d[which], stage, col0 + cb, row0, 0);
-            tma_store_commit();
-            if (out32) {
-              tma_store_wait_read0();
-              mbar_arrive(my_free);
-            } else {
-              tma_store_wait_read1();          // every store but this one has read its staging tile
-              if (n >= 1u) mbar_arrive(my_free + 8 * (sb ^ 1u));
-            }
-          }
-        }
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        __syncwarp();
       }
       // this warp has read the accumulator: the next tile but one may overwrite it
       tc_fence_before_sync();
-      if (ok) mbar_arrive_cluster_warp(leader_acc_empty + 8 * buf);
+      mbar_arrive_cluster_warp(leader_acc_empty + 8 * buf);
     }
-    if (storer) tma_store_wait_read0();
   }
 
   settle_if_aborted(s_abort);

@@ -15,9 +15,8 @@ enum ProductMode {
                     // of two products reduced over the tokens
 };
 
-// Operands and results.  kProductI8, kGated*: x[0] tokens, y weights (w_gate, w_up), d result (h, gate, up).
-// kGrad: x dgate and dup, y w_gate, w_up and the tokens, d dx, dw_gate and dw_up.
-struct ProductMaps { CUtensorMap x[2], y[3], d[3]; };
+// Operands.  kProductI8, kGated*: x[0] tokens, y weights (w_gate, w_up).  kGrad: x dgate and dup, y w_gate, w_up and the tokens.
+struct ProductMaps { CUtensorMap x[2], y[3]; };
 
 struct ProductParams {
   int rows, cols;          // of the result (kGrad: of dx)
@@ -29,8 +28,9 @@ struct ProductParams {
   const float* col_scale;  // of the channels (kGatedI8: of w_gate)
   const float* col_scale2; // kGatedI8: of w_up
   const float* bias;       // kProductI8, or null
-  void* d[3];              // results and the distance of their rows
+  void* d[3];              // results (kGated*: h, gate, up; kGrad: dx, dw_gate, dw_up) and the distance of their rows
   int64_t d_stride[3];
+  int wide;                // all rows of the results start at multiples of 32 bytes
   int* status;
 };
 

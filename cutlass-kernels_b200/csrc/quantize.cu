@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(256, U > 4 ? 2 : elem_bytes(SDT) == 2 ? 5 : 4)
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
       x[u][h].raw = make_uint4(0u, 0u, 0u, 0u);
-      if (t + u * G < nvec) x[u][h].raw = __ldg(s + (t + u * G) * NH + h);
+      if (t + u * G < nvec) x[u][h].raw = __ldcs(s + (t + u * G) * NH + h);
     }
   uint32_t m = 0u;
 #pragma unroll
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(256, U > 4 ? 2 : elem_bytes(SDT) == 2 ? 5 : 4)
     for (int h = 0; h < NH; ++h) m = max_pattern(m, x[u][h].raw, SB);
   for (int v = t + U * G; v < nvec; v += G) {
 #pragma unroll
-    for (int h = 0; h < NH; ++h) m = max_pattern(m, __ldg(s + v * NH + h), SB);
+    for (int h = 0; h < NH; ++h) m = max_pattern(m, s[v * NH + h], SB);
   }
   if constexpr (SB == 2) {                       // as fp32: the larger of the two
     ElemPack<SDT, 1> e;
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(256, U > 4 ? 2 : elem_bytes(SDT) == 2 ? 5 : 4)
   for (int v = t + U * G; v < nvec; v += G) {
     Half y[NH];
 #pragma unroll
-    for (int h = 0; h < NH; ++h) y[h].raw = __ldg(s + v * NH + h);
+    for (int h = 0; h < NH; ++h) y[h].raw = s[v * NH + h];
     store(v, y);
   }
   if (t < 8 && last < cols) d[last] = zero ? (int8_t)0 : (int8_t)quantize_by_division(tail, sc);

@@ -162,7 +162,7 @@ int cfk_gemm_plan(const cfk_gemm_args* args, int plan[3]);
  * The lengths themselves are free: any m, n, k >= 1.  Nothing is read or written behind the end of a row.  Outputs overlap no
  * input and no other output, unless a comment allows it.  Sums are exact (integers) or fp32; results are rounded once.
  * Pointers and stream belong to the current device.  No workspace but the status block (cfk_device_status reports a wait
- * that gave up, codes 211-216 and 221-224); calls can be captured.  Results do not depend on timing.  Which kernel a call
+ * that gave up, codes 211-214 and 221-223); calls can be captured.  Results do not depend on timing.  Which kernel a call
  * runs depends on its sizes and types (and, with it, the order of fp32 sums); integer sums do not depend on it.
  */
 
@@ -252,6 +252,16 @@ typedef struct cfk_ffn_gated_backward_args {
 } cfk_ffn_gated_backward_args;
 
 int cfk_ffn_gated_backward(const cfk_ffn_gated_backward_args* args, cfk_stream_t stream);
+
+/*
+ * Which kernel such a call would run, as cfk_fmha_plan and cfk_gemm_plan tell; launches nothing, needs no device.  plan[0] = 0: CTA pairs
+ * with tiles of 256 tokens (for the weights' gradients: 256 channels), 1: the kernel for few tokens; plan[1] = accumulator columns per
+ * CTA of a tile on pairs (64, 96, 128), or tokens per tile; plan[2] = CTAs that share a reduction.  Of the backward call these three
+ * are of dx (plan[1] = 0 without one), and plan[3] is the tile width of the weights' gradients (0 without them).
+ */
+int cfk_gemm_i8_plan(const cfk_gemm_i8_args* args, int plan[3]);
+int cfk_ffn_gated_plan(const cfk_ffn_gated_args* args, int plan[3]);
+int cfk_ffn_gated_backward_plan(const cfk_ffn_gated_backward_args* args, int plan[4]);
 
 /*
  * Device-side random fills, element i depends only on (seed, first_index + i).

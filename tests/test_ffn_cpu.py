@@ -1,5 +1,6 @@
 """Arguments that the feed-forward operators refuse, before they touch a device, and the layout of their structs."""
 import ctypes as C
+import random
 
 import pytest
 
@@ -51,7 +52,7 @@ def test_gemm_i8_refuses(lib, over, code):
     (dict(out_dtype=cfk.FP32), 1), (dict(activation=4), 1), (dict(activation=-1), 1), (dict(gate=0x5000), 1), (dict(up=0x5000), 1),
     (dict(x_scale=0x6000), 1), (dict(dtype=cfk.INT8), 1), (dict(dtype=cfk.INT8, x_scale=0x6000, gate_scale=0x7000), 1),
     (dict(x=0x1002), 1), (dict(w_gate=0x2008), 1), (dict(k=60), 1), (dict(x_stride=60, k=60), 1), (dict(n=60), 1),
-    (dict(gate=0x5000, up=0x6008), 1), (dict(gate=0x5000, up=0x6000, pre_stride=32), 1), (dict(h_stride=56), 1),
+    (dict(gate=0x5000, up=0x6008), 1), (dict(gate=0x5000, up=0x5000), 1), (dict(gate=0x4000, up=0x5000), 1), (dict(gate=0x5000, up=0x6000, pre_stride=32), 1), (dict(h_stride=56), 1),
     (dict(dtype=cfk.INT8, x_scale=0x6000, gate_scale=0x7000, up_scale=0x8000, k=131072), 2),
 ])
 def test_ffn_gated_refuses(lib, over, code):
@@ -79,6 +80,61 @@ def test_ffn_gated_backward_refuses(lib, over, code):
     order = ["dh", "x", "w_gate", "w_up", "gate", "up", "dgate", "dup"]
     assert refused(lib.ffn_gated_backward, *[kw.pop(o) for o in order], **kw) == code
     assert lib.lib.cfk_ffn_gated_backward(None, None) == 1
+
+
+P = list(range(0x1000, 0x10000, 0x1000))
+
+
+def product(m, n, k, out=cfk.BF16):
+    return cfk.GemmI8Args(out, m, n, k, P[0], P[1], P[2], P[3], P[4], None, 1 << 20, 1 << 20, 1 << 20)
+
+
+def gated(m, n, k, dtype=cfk.BF16):
+    scales = (P[4], P[5], P[6]) if dtype == cfk.INT8 else (None, None, None)
+    return cfk.FfnGatedArgs(dtype, cfk.BF16, 0, m, n, k, P[0], P[1], P[2], P[3], None, None, *scales, *[1 << 20] * 4)
+
+
+def backward(m, n, k, dx=True, dw=True):
+    return cfk.FfnGatedBackwardArgs(cfk.BF16, 0, m, n, k, *P[:8], P[8] if dx else None, *((P[9], P[10]) if dw else (None, None)),
+                                    *[1 << 20] * 7)
+
+
+def test_plans_can_be_run_and_cover_both_kernels(lib):
+    """Over sizes and types: tile widths and cluster sizes that the kernels have; few tokens go to the kernel for them, large products to
+    the CTA pairs; the plan does not depend on the output's type, addresses or strides."""
+    rng = random.Random(5)
+    log = lambda lo, hi: int(round(lo * (hi / lo) ** rng.random()))      # noqa: E731
+    seen = set()
+    for _ in range(3000):
+        m, n, k = log(1, 20000), log(1, 20000), log(1, 20000)
+        for args, widest in ((product(m, n, k), 256), (gated(m, n, k), 128), (gated(m, n, k, cfk.INT8), 128)):
+            few, width, parts = plan = lib.ffn_plan(args)
+            seen.add((widest, few))
+            if few:
+                assert width in (16, 32, 64, 128, 256) and width <= widest and (width == 16 or width < 2 * m)
+                assert parts in (1, 2, 3, 4, 6, 8)
+            else:
+                assert width in (64, 96, 128) and parts == 1
+            if m <= 4 and n >= 128:
+                assert few
+            if m * n >= 256 * 256 * 74 * 4 and m >= 2048 and k >= 512:
+                assert not few
+        assert lib.ffn_plan(product(m, n, k, cfk.FP32)) == lib.ffn_plan(product(m, n, k))
+        few, width, parts, dw = lib.ffn_plan(backward(m, n, k))
+        assert (width in (16, 32, 64, 128, 256) and parts in (1, 2, 3, 4, 6, 8)) if few else (width in (64, 96, 128) and parts == 1)
+        assert dw in (64, 96, 128)
+        assert lib.ffn_plan(backward(m, n, k, dx=False))[:3] == (0, 0, 1) and lib.ffn_plan(backward(m, n, k, dw=False))[3] == 0
+    assert seen == {(256, 0), (256, 1), (128, 0), (128, 1)}
+
+
+def test_plans_refuse_what_the_calls_refuse(lib):
+    for args in (product(0, 8, 8), gated(1, 0, 8), backward(1, 8, 0)):
+        with pytest.raises(cfk.CfkError) as e:
+            lib.ffn_plan(args)
+        assert e.value.code == 1
+    for name in ("cfk_gemm_i8_plan", "cfk_ffn_gated_plan", "cfk_ffn_gated_backward_plan"):
+        assert getattr(lib.lib, name)(None, None) == 1
+    assert lib.lib.cfk_gemm_i8_plan(C.byref(product(8, 8, 8)), None) == 1
 
 
 def test_int8_is_no_type_of_the_other_entry_points(lib):

@@ -1,5 +1,6 @@
 """The feed-forward operators against their definitions in 64 bits (bounds: ffn_helpers.py)."""
 import math
+import random
 
 import pytest
 import torch
@@ -336,6 +337,49 @@ def test_backward_far_pre_activations_are_finite(lib, cuda, act):
     check(dup, value, (half(cfk.BF16) + 3 * ACT_REL) * value.abs() + 1e-30)
 
 
+# ---- every cut -----------------------------------------------------------------------------------------------------------------------
+def smallest_of_every_plan(lib, args_of, seed, fewest):
+    """One shape, the smallest found, for every plan that random shapes get: kernel, tile width, parts of the reduction."""
+    rng = random.Random(seed)
+    log = lambda lo, hi: int(round(lo * (hi / lo) ** rng.random()))      # noqa: E731
+    best = {}
+    for _ in range(6000):
+        shape = log(1, 3000), log(8, 3000), log(8, 3000)
+        plan = lib.ffn_plan(args_of(*shape))
+        cost = shape[0] * shape[1] * shape[2]
+        if plan not in best or cost < best[plan][0]:
+            best[plan] = (cost, shape)
+    assert len(best) >= fewest and {p[0] for p in best} == {0, 1} and {p[1] for p in best if not p[0]} == {64, 96, 128}
+    return [shape for _, shape in best.values()]
+
+
+def packed_args(cls, *head):
+    """Arguments for a plan: valid made-up addresses and strides."""
+    at = [0x1000 * (i + 1) for i in range(11)]
+    if cls is cfk.GemmI8Args:
+        return lambda m, n, k: cls(cfk.FP16, m, n, k, *at[:5], None, *[1 << 20] * 3)
+    if cls is cfk.FfnGatedArgs:
+        scales = at[4:7] if head[0] == cfk.INT8 else [None] * 3
+        return lambda m, n, k: cls(head[0], cfk.FP16, 0, m, n, k, *at[:4], None, None, *scales, *[1 << 20] * 4)
+    return lambda m, n, k: cls(cfk.FP16, 0, m, n, k, *at, *[1 << 20] * 7)
+
+
+def test_every_cut_of_the_8_bit_product(lib, cuda):
+    for i, (m, n, k) in enumerate(smallest_of_every_plan(lib, packed_args(cfk.GemmI8Args), 1, 8)):
+        run_gemm_i8(lib, m, n, k, [cfk.FP16, cfk.BF16, cfk.FP32][i % 3], bias=i % 2 == 0, seed=i)
+
+
+@pytest.mark.parametrize("dtype", [cfk.FP16, cfk.INT8])
+def test_every_cut_of_the_gated_block(lib, cuda, dtype):
+    for i, (m, n, k) in enumerate(smallest_of_every_plan(lib, packed_args(cfk.FfnGatedArgs, dtype), 2, 7)):
+        run_gated(lib, dtype, cfk.FP16, ACTS[i % 4], m, n, k, keep=i % 2 == 0, seed=i)
+
+
+def test_every_cut_of_the_backward_pass(lib, cuda):
+    for i, (m, n, k) in enumerate(smallest_of_every_plan(lib, packed_args(cfk.FfnGatedBackwardArgs), 3, 20)):
+        run_backward(lib, cfk.FP16 if i % 2 else cfk.BF16, ACTS[i % 4], m, n, k, seed=i)
+
+
 # ---- together ------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("m", [1, 19, 300])
 def test_an_8_bit_block_end_to_end(lib, cuda, m):
@@ -471,6 +515,35 @@ def test_calls_on_several_streams_at_once(lib, cuda):
     lib.check_device()
     for (outs, _), w in zip(sets, want):
         assert all(torch.equal(o, x) for o, x in zip(outs, w))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 512, 1024), (5, 256, 256), (260, 256, 128)])
+def test_a_call_reads_what_the_launch_before_it_wrote(lib, cuda, m, n, k):
+    """New tokens every round, enqueued without a wait: fill -> quantise -> product and gated block, each launch set up while the ones
+    before still run.  Every round must give what it gives alone."""
+    rounds = 60
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    xq, sx = torch.zeros(m, k, dtype=torch.int8, device="cuda"), torch.zeros(m, device="cuda")
+    (wq, sw), wg, wu = quantized(gen(0), n, k), (randn(gen(1), n, k) / 9).bfloat16(), (randn(gen(2), n, k) / 9).bfloat16()
+
+    def one(seed, y, h, stream):
+        lib.fill(x, cfk.BF16, m * k, seed, scale=1.0 + seed % 7, stream=stream)
+        lib.quantize_rows(x, xq, sx, src_dtype=cfk.BF16, rows=m, cols=k, stream=stream)
+        lib.gemm_i8(xq, wq, y, m=m, n=n, k=k, out_dtype=cfk.FP32, a_scale=sx, b_scale=sw, stream=stream)
+        lib.ffn_gated(x, wg, wu, h, dtype=cfk.BF16, out_dtype=cfk.BF16, activation=cfk.ACT_SILU, m=m, n=n, k=k, stream=stream)
+
+    shape = (rounds, m, n)
+    y0, y1 = torch.zeros(shape, device="cuda"), torch.zeros(shape, device="cuda")
+    h0, h1 = torch.zeros(shape, dtype=torch.bfloat16, device="cuda"), torch.zeros(shape, dtype=torch.bfloat16, device="cuda")
+    for i in range(rounds):
+        one(i, y0[i], h0[i], None)
+        lib.check_device()
+    stream = torch.cuda.Stream()
+    for i in range(rounds):
+        one(i, y1[i], h1[i], stream.cuda_stream)
+    lib.check_device()
+    assert torch.equal(y0, y1) and torch.equal(h0, h1)
+    assert len({float(v) for v in y0.abs().amax((1, 2))}) > rounds // 2       # the rounds differ
 
 
 def test_offsets_beyond_32_bits(lib, cuda):
