@@ -8,6 +8,7 @@
 #include "element_io.cuh"
 #include "ffn_act.cuh"
 #include "ffn_params.h"
+#include "gemm_tiles.cuh"
 #include "host_util.h"
 
 namespace cfk {
@@ -280,7 +281,17 @@ static int run_few(const ProductCall& c, const FewPlan& few, cudaStream_t stream
 }
 
 template <int MODE>
-static int run_pairs(const ProductCall& c, const PairPlan& plan, cudaStream_t stream) {
+static int run_pairs(const ProductCall& c, PairPlan plan, cudaStream_t stream) {
+  const int first = plan.job[0].tiles_r * plan.job[0].tiles_c * plan.job[0].batches;
+  plan.most = first / plan.pairs;
+  plan.more = first % plan.pairs;
+  plan.staged = MODE == kGrad && plan.job[plan.jobs - 1].kind == 1 && plan.job[plan.jobs - 1].reduce <= 512;   // weights' gradients
+  for (int i = 0; i < plan.jobs; ++i) {
+    PairJob& j = plan.job[i];
+    j.per_batch = make_divisor((uint32_t)(j.tiles_r * j.tiles_c));
+    j.per_band = make_divisor((uint32_t)(kGemmBand * j.tiles_c));
+    j.tail_rows = make_divisor((uint32_t)(j.tiles_r % kGemmBand ? j.tiles_r % kGemmBand : 1));
+  }
   ProductParams p = c.p;
   ProductMaps maps;
   std::memset(&maps, 0, sizeof(maps));

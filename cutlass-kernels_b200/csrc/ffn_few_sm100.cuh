@@ -313,15 +313,8 @@ few_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_consta
 
 template <int MODE>
 int launch_few_product(const ProductMaps& maps, const ProductParams& p, const FewPlan& f, cudaStream_t stream) {
-  static thread_local int attr_dev = -1;
-  int dev = 0;
-  if (note_cuda(cudaGetDevice(&dev), "cudaGetDevice") != cudaSuccess) return CFK_ERR_NO_DRIVER;
-  if (attr_dev != dev) {
-    if (note_cuda(cudaFuncSetAttribute(few_product_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmemFull),
-                  "cudaFuncSetAttribute(few-token smem)") != cudaSuccess)
-      return CFK_ERR_LAUNCH;
-    attr_dev = dev;
-  }
+  const int rc = allow_shared_memory(few_product_kernel<MODE>, kFewSmemFull);
+  if (rc) return rc;
   const dim3 grid((unsigned)(f.tiles_ch * f.tiles_tok * f.splits));
   const size_t smem = kFewHead + (size_t)f.stages * (few_weights(MODE) * FewCfg::WB + f.tt * 128);
   return note_cuda(launch_overlapped_in(f.splits, few_product_kernel<MODE>, grid, dim3(FewCfg::NTHREADS), smem, stream, maps, p, f),

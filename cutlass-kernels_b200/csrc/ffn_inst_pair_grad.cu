@@ -1,4 +1,4 @@
 #include "ffn_pair_sm100.cuh"
 namespace cfk {
-template int launch_pair_product<kGrad>(const ProductMaps&, const ProductParams&, const PairPlan&, cudaStream_t);
+template int launch_pair_product<kGrad>(const ProductMaps&, const ProductParams&, PairPlan, cudaStream_t);
 }

@@ -11,9 +11,9 @@
 //                operand is contiguous: both are MN-major.
 //
 // Roles, ring and tensor-memory double buffer are those of gemm_kernel: warp 0 TMA, warp 1 of the leader UMMA (cta_group::2); but
-// two groups of four epilogue warps, which write whole sectors from registers.  (A TMA store writes whole 16-byte pieces, so behind
-// the last element of a row it would put zeros up to the next multiple of 16 bytes; and the hand-over of its staging tiles took 0.6 us
-// per 32 columns, most of a tile whose reduction is short.)
+// two groups of four epilogue warps, which write with ordinary stores.  (A TMA store writes whole 16-byte pieces, so behind the last element
+// of a row it would put zeros up to the next multiple of 16 bytes; and the hand-over of staging tiles between four warps and a
+// storing thread took 0.6 us per 32 columns, most of a tile whose reduction is short.)
 // An MN-major operand lands as spans of 64 columns, [span][64 k-rows][128 bytes], each with the 128-byte swizzle; what lies
 // behind a matrix is zero-filled in both operands, so ragged reductions need no mask.
 //
@@ -33,16 +33,17 @@ constexpr int kErrPairFull = 211, kErrPairEmpty = 212, kErrPairAccFull = 213, kE
 
 struct PairCfg {
   static constexpr int TM = 256, TN = 256, BM = 128, BN = 128;     // tile of the pair; rows of X and of Y per CTA
-  static constexpr int XB = BM * 128, YB = BN * 128;               // bytes per k-block
-  static constexpr int NSTAGE = 7;
+  static constexpr int XB = BM * 128, SPANB = 64 * 128;            // bytes per k-block: of X; of a 64 x 64 box of an MN-major operand
   static constexpr int GROUPS = 2;                                 // of four epilogue warps
-  static constexpr int SMEM_BYTES = 1024 + NSTAGE * (XB + YB) + 256;
+  static constexpr int HEADB = 1024 + 256, MAXSTAGE = 8;           // alignment slack and the barrier block
+  static constexpr int STAGEB = 32 * 128;                          // output staging of an epilogue warp, where results are staged
   static constexpr int NTHREADS = 64 + GROUPS * 128;
-  static_assert(8 * (2 * NSTAGE + 4) + 8 <= 256, "barrier block overflows");
+  static_assert(8 * (2 * MAXSTAGE + 4) + 8 <= 256, "barrier block overflows");
 };
 
-// 32 columns of a row, from `col` on, as far as they exist.  A thread writes whole 32-byte sectors where rows start at multiples of
-// 32 bytes (`wide`), and nothing behind the row's end.
+// Results leave in one of two ways.
+// From registers: a thread has a row and writes 32 columns of it, in whole 32-byte sectors where rows start at multiples of 32 bytes
+// (`wide`), and nothing behind the row's end.
 __device__ __forceinline__ void st_global_32(void* to, const uint32_t (&w)[32], int at) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[at]), "r"(w[at + 1]), "r"(w[at + 2]),
                "r"(w[at + 3]), "r"(w[at + 4]), "r"(w[at + 5]), "r"(w[at + 6]), "r"(w[at + 7]) : "memory");
@@ -91,6 +92,51 @@ __device__ __forceinline__ void store_columns(const ProductParams& p, int which,
   }
 }
 
+// Through shared memory of each epilogue warp, 32 rows x 128 bytes (64 columns): 8 threads per row, so that an instruction writes whole
+// lines and not a sector of 32 of them.  0.7 us per 64 columns of a tile instead of 0.9, at the price of a stage of the ring: taken for
+// gradients of the weights from up to 512 tokens, which are little but writes (5632 x 2048 from 64 tokens: 16.7 us against 18.1; 2048 x 4096 from
+// 300: 17.8 / 18.7; 2731 x 1027 from 777: 19.5 / 19.1); elsewhere the stage is worth more (8-bit products of 1500 x 4096 x 1024: 13.7
+// against 12.2).  The pieces of a row are exchanged by the row's index, against bank conflicts.
+__device__ __forceinline__ uint32_t staged_at(uint32_t tile, int r, int piece) { return tile + r * 128 + ((piece ^ (r & 7)) << 4); }
+__device__ __forceinline__ void stage_columns(uint32_t tile, int r, int piece0, bool bf16, const float (&v)[32]) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const uint32_t w0 = pack_out(bf16, v[g * 8], v[g * 8 + 1]), w1 = pack_out(bf16, v[g * 8 + 2], v[g * 8 + 3]);
+    const uint32_t w2 = pack_out(bf16, v[g * 8 + 4], v[g * 8 + 5]), w3 = pack_out(bf16, v[g * 8 + 6], v[g * 8 + 7]);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staged_at(tile, r, piece0 + g)), "r"(w0), "r"(w1), "r"(w2), "r"(w3)
+                 : "memory");
+  }
+}
+// The staged rows (first: `row`) to result `which` from column `col` on, as far as rows and columns exist.  The whole warp calls.
+__device__ __forceinline__ void store_staged(const ProductParams& p, int which, uint32_t tile, int row, int rows, int col, int cols) {
+  __syncwarp();
+  const int lane = threadIdx.x & 31, piece = lane & 7;
+  const int n = cols - (col + piece * 8);                 // columns of this thread's piece that exist, if fewer than 8
+  uint16_t* d = reinterpret_cast<uint16_t*>(p.d[which]) + (row + (lane >> 3)) * p.d_stride[which] + col + piece * 8;
+  const int64_t step = 4 * p.d_stride[which];
+#pragma unroll
+  for (int i = 0; i < 8; ++i, d += step) {
+    const int r = i * 4 + (lane >> 3);
+    if (row + r >= rows || n <= 0) continue;
+    uint32_t w[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(staged_at(tile, r, piece)) : "memory");
+    if (n >= 8) {
+      *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 7; ++e)
+        if (e < n) d[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+    }
+  }
+  __syncwarp();                                           // the staging may be written again
+}
+
+// int32 sums (as bit patterns) to scaled fp32; lane i holds the scale of column i
+__device__ __forceinline__ void scale_columns(float (&v)[32], float row_scale, float col_scale) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __int2float_rn(__float_as_int(v[i])) * row_scale * __shfl_sync(0xffffffffu, col_scale, i);
+}
 // h = act(gate) * up in place of gate
 template <int ACT>
 __device__ __forceinline__ void gate_by(float (&gate)[32], const float (&up)[32]) {
@@ -110,21 +156,34 @@ __device__ __forceinline__ void gate_columns(int act, float (&gate)[32], const f
 struct PairTile {
   int kind, tr, tc, batch, bn, rows, cols, nkb_part, nkb;
 };
-// The `local`-th tile of a pair; false: it has no more (see PairPlan for the order).
+__device__ __forceinline__ int divide(int n, const Divisor& d) { return (int)((__umulhi((uint32_t)n, d.m) + (uint32_t)n) >> d.shift); }
+// The `local`-th tile of a pair; false: it has no more (see PairPlan for the order).  Within a list the order is that of tile_coords
+// (gemm_tiles.cuh), with the divisions prepared on the host: 4 of them took a third of a microsecond per tile.
 __device__ __forceinline__ bool pair_tile(PairTile& t, const PairPlan& plan, int pair, int local, bool grad, int kb) {
-  const int first = plan.job[0].tiles_r * plan.job[0].tiles_c * plan.job[0].batches, pairs = plan.pairs;
-  const int mine = first > pair ? (first - pair + pairs - 1) / pairs : 0;
-  int j = 0, tile = pair + local * pairs;
+  const bool has_more = pair < plan.more;
+  const int mine = plan.most + (has_more ? 1 : 0);
+  int j = 0, tile = pair + local * plan.pairs;
   if (local >= mine) {
     if (plan.jobs < 2) return false;
-    const int i = local - mine, more = first % pairs;
+    const int i = local - mine;
     j = 1;
-    tile = pair < more ? i * more + pair : more * plan.share + i * (pairs - more) + (pair - more);
-    if (pair < more ? i >= plan.share : tile >= plan.job[1].tiles_r * plan.job[1].tiles_c * plan.job[1].batches) return false;
+    tile = has_more ? i * plan.more + pair : plan.more * plan.share + i * (plan.pairs - plan.more) + (pair - plan.more);
+    if (has_more ? i >= plan.share : tile >= plan.job[1].tiles_r * plan.job[1].tiles_c * plan.job[1].batches) return false;
   }
   const PairJob& job = plan.job[j];
   t.kind = job.kind; t.bn = job.bn; t.rows = job.rows; t.cols = job.cols;
-  tile_coords(tile, job.tiles_r, job.tiles_c, t.tr, t.tc, t.batch);
+  t.batch = divide(tile, job.per_batch);
+  int at = tile - t.batch * job.tiles_r * job.tiles_c;
+  const int band = divide(at, job.per_band), first_r = band * kGemmBand;
+  at -= band * kGemmBand * job.tiles_c;
+  if (job.tiles_r - first_r >= kGemmBand) {
+    t.tc = at / kGemmBand;
+    t.tr = first_r + at % kGemmBand;
+  } else {
+    t.tc = divide(at, job.tail_rows);
+    t.tr = first_r + at - t.tc * (job.tiles_r - first_r);
+  }
+  if (band & 1) t.tc = job.tiles_c - 1 - t.tc;
   t.nkb_part = (job.reduce + kb - 1) / kb;
   t.nkb = grad && t.kind == 0 ? 2 * t.nkb_part : t.nkb_part;
   return true;
@@ -142,14 +201,15 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
   const uint32_t sX = smem_base;
-  const uint32_t sY = smem_base + C::NSTAGE * C::XB;
-  const uint32_t sBar = sY + C::NSTAGE * C::YB;
-  const uint32_t bar_full = sBar;                            // [NSTAGE] leader: both CTAs' loads of a stage landed
-  const uint32_t bar_empty = sBar + 8 * C::NSTAGE;           // [NSTAGE] each CTA: its stage was consumed
-  const uint32_t bar_acc_full = bar_empty + 8 * C::NSTAGE;   // [2] each CTA: accumulator complete
+  const uint32_t ring_bytes = C::XB + plan.y_bytes;           // a k-block: X, then Y
+  const uint32_t sStage = sX + plan.stages * ring_bytes;     // [epilogue warps], where results are staged
+  const uint32_t sBar = sStage + (GRAD && plan.staged ? 4 * C::GROUPS * C::STAGEB : 0);
+  const uint32_t bar_full = sBar;                            // [stages] leader: both CTAs' loads of a stage landed
+  const uint32_t bar_empty = sBar + 8 * C::MAXSTAGE;         // [stages] each CTA: its stage was consumed
+  const uint32_t bar_acc_full = bar_empty + 8 * C::MAXSTAGE; // [2] each CTA: accumulator complete
   const uint32_t bar_acc_empty = bar_acc_full + 16;          // [2] leader: all epilogue warps of both have read it
   uint8_t* gBar = smem_gen + (sBar - smem_base);
-  const uint32_t off_misc = 8 * (2 * C::NSTAGE + 4);
+  const uint32_t off_misc = 8 * (2 * C::MAXSTAGE + 4);
   volatile uint32_t* s_tmem_base = reinterpret_cast<volatile uint32_t*>(gBar + off_misc);
   volatile uint32_t* s_abort = reinterpret_cast<volatile uint32_t*>(gBar + off_misc + 4);
   const AbortCtx actx{s_abort, p.status};
@@ -161,7 +221,7 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
 
   cluster_arrive_started();
   if (tid == 0) {
-    for (int i = 0; i < C::NSTAGE; ++i) { mbar_init(bar_full + 8 * i, 2); mbar_init(bar_empty + 8 * i, 1); }
+    for (int i = 0; i < plan.stages; ++i) { mbar_init(bar_full + 8 * i, 2); mbar_init(bar_empty + 8 * i, 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(bar_acc_full + 8 * i, 1); mbar_init(bar_acc_empty + 8 * i, 2 * 4 * C::GROUPS); }
     *s_abort = 0u;
     fence_barrier_init();
@@ -186,34 +246,34 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
 
   if (warp == 0) {
     if (lane == 0) {
-      int idx = 0, local = 0;
+      int s = 0, local = 0;
+      uint32_t ph = 0;
       bool ok = true;
       for (PairTile t; ok && pair_tile(t, plan, pair_id, local, GRAD, KB); ++local) {
         const int xr = t.tr * C::TM + (int)rank * C::BM;                                    // first of this CTA's rows of X
         const int yr = GATED ? t.tc * t.bn : t.tc * 2 * t.bn + (int)rank * t.bn;            // and of Y
-        const uint32_t bytes = C::XB + (GRAD ? (t.bn > 64 ? C::YB : C::YB / 2) : t.bn * 128);
-        for (int i = 0; i < t.nkb; ++i, ++idx) {
+        const uint32_t bytes = C::XB + (GRAD ? (t.bn > 64 ? 2 : 1) * C::SPANB : t.bn * 128);
+        for (int i = 0; i < t.nkb; ++i) {
           // every other tile walks the reduction backwards, from the k-blocks that are still in L2 (gemm_sm100.cu)
           const int kb = (local & 1) ? t.nkb - 1 - i : i;
           const int part = GRAD && kb >= t.nkb_part ? 1 : 0;
           const int k = (kb - part * t.nkb_part) * KB;
-          const int s = idx % C::NSTAGE;
-          const uint32_t ph = (idx / C::NSTAGE) & 1;
           if (!mbar_wait(bar_empty + 8 * s, ph ^ 1u, actx, kErrPairEmpty)) { ok = false; break; }
           const uint32_t full = map_to_cta(bar_full + 8 * s, 0);
-          const uint32_t x = sX + s * C::XB, y = sY + s * C::YB;
+          const uint32_t x = sX + s * ring_bytes, y = x + C::XB;
           mbar_arrive_expect_tx_cluster(full, bytes);
           if constexpr (GRAD) {      // boxes of 64 x 64
             const CUtensorMap* mx = &maps.x[t.kind == 0 ? part : t.batch];
             const CUtensorMap* my = &maps.y[t.kind == 0 ? part : 2];
             tma_load_3d_pair(x, mx, full, t.kind == 0 ? k : xr, t.kind == 0 ? xr : k, 0);
-            tma_load_3d_pair(x + C::XB / 2, mx, full, t.kind == 0 ? k : xr + 64, t.kind == 0 ? xr + 64 : k, 0);
+            tma_load_3d_pair(x + C::SPANB, mx, full, t.kind == 0 ? k : xr + 64, t.kind == 0 ? xr + 64 : k, 0);
             tma_load_3d_pair(y, my, full, yr, k, 0);
-            if (t.bn > 64) tma_load_3d_pair(y + C::YB / 2, my, full, yr + 64, k, 0);
+            if (t.bn > 64) tma_load_3d_pair(y + C::SPANB, my, full, yr + 64, k, 0);
           } else {
             tma_load_3d_pair(x, &maps.x[0], full, k, xr, 0);
             tma_load_3d_pair(y, &maps.y[GATED ? (int)rank : 0], full, k, yr, 0);
           }
+          if (++s == plan.stages) { s = 0; ph ^= 1u; }
         }
       }
     }
@@ -222,25 +282,25 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
     if (rank == 0) {
       const uint32_t leader = elect_one();
       const uint32_t fmt = p.bf16 ? kFmtBF16 : kFmtF16;
-      int idx = 0, local = 0;
+      int s = 0, local = 0;
+      uint32_t ph = 0;
       bool ok = true;
       for (PairTile t; ok && pair_tile(t, plan, pair_id, local, GRAD, KB); ++local) {
         const bool x_mn = GRAD && t.kind == 1;
         const uint32_t idesc = I8 ? make_idesc(2, kFmtS8, kFmtS8, 0, 0, C::TM, 2 * t.bn)
                                   : make_idesc(1, fmt, fmt, x_mn ? 1 : 0, GRAD ? 1 : 0, C::TM, 2 * t.bn);
         // 32 bytes along the reduction, or 16 rows of 128 bytes, per instruction
-        const uint32_t xstep = x_mn ? 2048 : 32, xlbo = x_mn ? C::XB / 2 : 16;
-        constexpr uint32_t YSTEP = GRAD ? 2048 : 32, YLBO = GRAD ? C::YB / 2 : 16;
+        const uint32_t xstep = x_mn ? 2048 : 32, xlbo = x_mn ? C::SPANB : 16;
+        constexpr uint32_t YSTEP = GRAD ? 2048 : 32, YLBO = GRAD ? C::SPANB : 16;
         const int buf = local & 1;
         if (!mbar_wait_warp(bar_acc_empty + 8 * buf, ((local >> 1) & 1) ^ 1u, actx, kErrPairAccEmpty)) { ok = false; break; }
         tc_fence_after_sync();
         const uint32_t d = tmem_base + buf * C::TN;
-        for (int i = 0; i < t.nkb; ++i, ++idx) {
-          const int s = idx % C::NSTAGE;
-          if (!mbar_wait_warp(bar_full + 8 * s, (idx / C::NSTAGE) & 1, actx, kErrPairFull)) { ok = false; break; }
+        for (int i = 0; i < t.nkb; ++i) {
+          if (!mbar_wait_warp(bar_full + 8 * s, ph, actx, kErrPairFull)) { ok = false; break; }
           tc_fence_after_sync();
-          const uint64_t a0 = make_smem_desc(sX + s * C::XB, xlbo, 1024, kSwizzle128B);
-          const uint64_t b0 = make_smem_desc(sY + s * C::YB, YLBO, 1024, kSwizzle128B);
+          const uint64_t a0 = make_smem_desc(sX + s * ring_bytes, xlbo, 1024, kSwizzle128B);
+          const uint64_t b0 = make_smem_desc(sX + s * ring_bytes + C::XB, YLBO, 1024, kSwizzle128B);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
             const uint64_t a = desc_advance(a0, kk * xstep), bd = desc_advance(b0, kk * YSTEP);
@@ -248,23 +308,26 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
             else umma_ss_e<false, true>(d, a, bd, idesc, (i | kk) != 0 ? 1u : 0u, leader);
           }
           umma_commit_pair_e(bar_empty + 8 * s, (uint16_t)3, leader);      // the stage is free in both CTAs
+          if (++s == plan.stages) { s = 0; ph ^= 1u; }
         }
         if (ok) umma_commit_pair_e(bar_acc_full + 8 * buf, (uint16_t)3, leader);
       }
     }
   } else {
-    // epilogue warps 2..9 in two groups of four, which take 32 columns of the tile in turn; warp w may touch TMEM lanes
-    // 32*(w%4) .. +31, a row per thread.
+    // epilogue warps 2..9 in two groups of four, which take 32 columns of the tile in turn (64 where they are staged); warp w may
+    // touch TMEM lanes 32*(w%4) .. +31, a row per thread.
     const int grp = (warp - 2) >> 2;
     const int q = warp & 3;
-    const int r = q * 32 + lane;                       // row within this CTA's 128 rows
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     const uint32_t leader_acc_empty = map_to_cta(bar_acc_empty, 0);
+    const uint32_t stage = sStage + (warp - 2) * C::STAGEB;
+    const bool staged = GRAD && plan.staged;
+    const int step = staged ? 64 : 32;
     int local = 0;
     bool ok = true;
     for (PairTile t; ok && pair_tile(t, plan, pair_id, local, GRAD, KB); ++local) {
       const int buf = local & 1;
-      const int row = t.tr * C::TM + (int)rank * C::BM + r;
+      const int row0 = t.tr * C::TM + (int)rank * C::BM + q * 32, row = row0 + lane;
       const int tcols = GATED ? t.bn : 2 * t.bn, col0 = t.tc * tcols;
       const int end = t.cols - col0 < tcols ? t.cols - col0 : tcols;     // columns of the tile that exist
       const uint32_t acc = tmem_base + lane_base + buf * C::TN;
@@ -275,27 +338,20 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
       if (!ok) break;
       tc_fence_after_sync();
 #pragma unroll 1
-      for (int cb = grp * 32; cb < end; cb += C::GROUPS * 32) {
+      for (int cb = grp * step; cb < end; cb += C::GROUPS * step) {
         const int col = col0 + cb, mine = col + lane;          // this lane's column: its scales reach the others by shuffle
         float v[32];
         if constexpr (GATED) {
           float u[32];
-          uint32_t w[32], x[32];
-          tmem_ld_x32(acc + cb, w);
-          tmem_ld_x32(acc + t.bn + cb, x);
+          tmem_ld_x32(acc + cb, reinterpret_cast<uint32_t*>(v));
+          tmem_ld_x32(acc + t.bn + cb, reinterpret_cast<uint32_t*>(u));
           if constexpr (I8) {
-            const float gs = mine < t.cols ? p.col_scale[mine] : 0.f;
-            const float us = mine < t.cols ? p.col_scale2[mine] : 0.f;
+            const float gs = mine < t.cols ? p.col_scale[mine] : 0.f, us = mine < t.cols ? p.col_scale2[mine] : 0.f;
             tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              v[i] = __int2float_rn((int)w[i]) * rs * __shfl_sync(0xffffffffu, gs, i);
-              u[i] = __int2float_rn((int)x[i]) * rs * __shfl_sync(0xffffffffu, us, i);
-            }
+            scale_columns(v, rs, gs);
+            scale_columns(u, rs, us);
           } else {
             tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) { v[i] = __uint_as_float(w[i]); u[i] = __uint_as_float(x[i]); }
           }
           if (p.keep && inside) {
             store_columns(p, 1, row, col, t.cols, v);
@@ -303,25 +359,27 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
           }
           gate_columns(p.act, v, u);
           if (inside) store_columns(p, 0, row, col, t.cols, v);
-        } else {
-          uint32_t w[32];
-          tmem_ld_x32(acc + cb, w);
-          if constexpr (I8) {
-            const float cs = mine < t.cols ? p.col_scale[mine] : 0.f;
-            const float bs = p.bias != nullptr && mine < t.cols ? p.bias[mine] : 0.f;
-            tmem_wait_ld();
+        } else if constexpr (I8) {
+          tmem_ld_x32(acc + cb, reinterpret_cast<uint32_t*>(v));
+          const float cs = mine < t.cols ? p.col_scale[mine] : 0.f;
+          const float bs = p.bias != nullptr && mine < t.cols ? p.bias[mine] : 0.f;
+          tmem_wait_ld();
+          scale_columns(v, rs, cs);
+          if (p.bias != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __int2float_rn((int)w[i]) * rs * __shfl_sync(0xffffffffu, cs, i);
-            if (p.bias != nullptr) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, bs, i);
-            }
-          } else {
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(w[i]);
+            for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, bs, i);
           }
-          if (inside) store_columns(p, GRAD ? (t.kind == 0 ? 0 : 1 + t.batch) : 0, row, col, t.cols, v);
+          if (inside) store_columns(p, 0, row, col, t.cols, v);
+        } else {
+          const int which = t.kind == 0 ? 0 : 1 + t.batch;
+#pragma unroll 1
+          for (int h = 0; h < step && cb + h < end; h += 32) {
+            tmem_ld_x32(acc + cb + h, reinterpret_cast<uint32_t*>(v));
+            tmem_wait_ld();
+            if (staged) stage_columns(stage, lane, h / 8, p.bf16, v);
+            else if (inside) store_columns(p, which, row, col, t.cols, v);
+          }
+          if (staged) store_staged(p, which, stage, row0, t.rows, col, end - cb < 64 ? col0 + end : col + 64);
         }
         __syncwarp();
       }
@@ -342,20 +400,21 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
 }
 
 template <int MODE>
-int launch_pair_product(const ProductMaps& maps, const ProductParams& p, const PairPlan& plan, cudaStream_t stream) {
+int launch_pair_product(const ProductMaps& maps, const ProductParams& p, PairPlan plan, cudaStream_t stream) {
   using C = PairCfg;
-  static thread_local int attr_dev = -1;
-  int dev = 0;
-  if (note_cuda(cudaGetDevice(&dev), "cudaGetDevice") != cudaSuccess) return CFK_ERR_NO_DRIVER;
-  if (attr_dev != dev) {
-    if (note_cuda(cudaFuncSetAttribute(pair_product_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES),
-                  "cudaFuncSetAttribute(product smem)") != cudaSuccess)
-      return CFK_ERR_LAUNCH;
-    attr_dev = dev;
-  }
-  return note_cuda(launch_overlapped_in(2, pair_product_kernel<MODE>, dim3((unsigned)(2 * plan.pairs)), dim3(C::NTHREADS),
-                                        C::SMEM_BYTES, stream, maps, p, plan), "product launch") == cudaSuccess ? CFK_OK
-                                                                                                                : CFK_ERR_LAUNCH;
+  constexpr int SMEM = 227 * 1024 - 128;                  // and a few static bytes of the kernel
+  const int rc = allow_shared_memory(pair_product_kernel<MODE>, SMEM);
+  if (rc) return rc;
+  // narrower tiles leave room for more stages
+  int bn = plan.job[0].bn;
+  if (plan.jobs > 1 && plan.job[1].bn > bn) bn = plan.job[1].bn;
+  plan.y_bytes = MODE == kGrad ? (bn > 64 ? 2 : 1) * C::SPANB : bn * 128;
+  const int head = C::HEADB + (MODE == kGrad && plan.staged ? 4 * C::GROUPS * C::STAGEB : 0);
+  plan.stages = (SMEM - head) / (C::XB + plan.y_bytes);
+  if (plan.stages > C::MAXSTAGE) plan.stages = C::MAXSTAGE;
+  const size_t smem = head + (size_t)plan.stages * (C::XB + plan.y_bytes);
+  return note_cuda(launch_overlapped_in(2, pair_product_kernel<MODE>, dim3((unsigned)(2 * plan.pairs)), dim3(C::NTHREADS), smem,
+                                        stream, maps, p, plan), "product launch") == cudaSuccess ? CFK_OK : CFK_ERR_LAUNCH;
 }
 
 }  // namespace cfk

@@ -34,6 +34,17 @@ struct ProductParams {
   int* status;
 };
 
+// Division of 0 <= n < 2^31 by a constant of the launch: a product and a shift (T. Granlund, P. Montgomery, Division by invariant
+// integers using multiplication, 1994).
+struct Divisor {
+  uint32_t m, shift;
+};
+inline Divisor make_divisor(uint32_t d) {
+  uint32_t l = 0;
+  while (l < 31 && (1u << l) < d) ++l;
+  return Divisor{(uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << l) - d)) / d + 1), l};
+}
+
 // One list of output tiles of the kernel on CTA pairs (256 rows x 2 bn accumulator columns each).
 struct PairJob {
   int kind;                // kGrad: 0 dx, 1 dw_gate and dw_up
@@ -41,13 +52,20 @@ struct PairJob {
   int reduce;              // of a part of the reduction
   int bn;                  // accumulator columns per CTA: 64, 96 or 128.  A tile has bn columns of h, 2 bn of any other result
   int tiles_r, tiles_c, batches;
+  Divisor per_batch, per_band, tail_rows;      // tiles of a batch, of a band of kGemmBand tile rows; tile rows of the last, shorter band
 };
 // The pairs take the tiles of the first list in turn.  Those that get one more of them than the others take `share` tiles of the second
 // list each, the others what is left.
-struct PairPlan { PairJob job[2]; int jobs, pairs, share; };
+struct PairPlan {
+  PairJob job[2];
+  int jobs, pairs, share;
+  int most, more;          // tiles of the first list that every pair has; pairs that have one more
+  int stages, y_bytes;     // of the ring; of a k-block of Y in a stage
+  int staged;              // kGrad: results pass through shared memory
+};
 
 template <int MODE>
-int launch_pair_product(const ProductMaps& maps, const ProductParams& p, const PairPlan& plan, cudaStream_t stream);
+int launch_pair_product(const ProductMaps& maps, const ProductParams& p, PairPlan plan, cudaStream_t stream);
 
 // How the kernel for few tokens cuts a product (kGrad: dx).
 struct FewPlan {

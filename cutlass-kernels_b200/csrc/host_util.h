@@ -44,6 +44,23 @@ inline cudaError_t launch_overlapped(void (*kern)(KArgs...), dim3 grid, dim3 blo
   return launch_overlapped_in(1, kern, grid, block, smem, stream, args...);
 }
 
+// Allows a kernel `bytes` of dynamic shared memory on the current device; asked once per thread and device.  Internal linkage: the
+// record belongs to the kernel of this copy of the library.
+template <class... KArgs>
+static int allow_shared_memory(void (*kern)(KArgs...), int bytes) {
+  static thread_local const void* kernel = nullptr;       // a translation unit instantiates this for one kernel or a few
+  static thread_local int device = -1;
+  int dev = 0;
+  if (note_cuda(cudaGetDevice(&dev), "cudaGetDevice") != cudaSuccess) return CFK_ERR_NO_DRIVER;
+  if (device == dev && kernel == reinterpret_cast<const void*>(kern)) return CFK_OK;
+  if (note_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                "cudaFuncSetAttribute(shared memory)") != cudaSuccess)
+    return CFK_ERR_LAUNCH;
+  device = dev;
+  kernel = reinterpret_cast<const void*>(kern);
+  return CFK_OK;
+}
+
 // SMs of the one device this library is built for.  Only the choice between kernels and the sizes of grids follow from it.
 constexpr int kSMs = 148;
 
