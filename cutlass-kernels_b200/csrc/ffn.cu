@@ -78,15 +78,21 @@ static cudaError_t launch_gate_grad(const cfk_ffn_gated_backward_args* a, cudaSt
 }
 
 // ---- cuts -------------------------------------------------------------------------------------------------------------------
-// Which kernel and which tiles follows from estimates of its time, in us, whose constants are fits to a sweep of 240 shapes (1 to
-// 3000 tokens, widths 128 to 11264 and 8192) x all cuts: root mean square error 7 to 13 %, and the cut they choose is on average
-// within 2 % of the best one measured, at worst 35 %.
+// Which kernel and which tiles follows from estimates of its time, in us, whose constants are fits to a sweep of 1170 calls (1 to 16000
+// tokens, widths 128 to 16384 and 8192) x all cuts: root mean square error 8 to 15 %.  The cut they choose is 1 to 4 % slower than the
+// best one measured, on average over the calls of a kind, and 31 % at worst.
 constexpr int kPairs = kSMs / 2;
 
 static bool is_gated(int mode) { return mode == kGated16 || mode == kGatedI8; }
 static int k_blocks(int mode, int reduce) {
   const int kb = mode == kProductI8 || mode == kGatedI8 ? 128 : 64;
   return (reduce + kb - 1) / kb;
+}
+
+// Three things that run beside each other take the longest one's time and some of the others'.
+static float overlapped(float a, float b, float c) {
+  const float most = fmaxf(a, fmaxf(b, c));
+  return most + 0.22f * (a + b + c - most);
 }
 
 // Clusters of 1, 2, 3, 4, 6 and 8 CTAs that are resident at once, with one and with two CTAs per SM, as
@@ -99,7 +105,7 @@ constexpr int kResident[2][6] = {{148, 74, 45, 33, 22, 15}, {296, 148, 93, 71, 4
 // ring where the clusters fit that way: one gated token of 11264 x 4096 bf16 32.0 us against 36.2 with half of it.
 static float plan_few(int mode, int rows, int cols, int reduce, FewPlan* best) {
   const int nw = few_weights(mode), nkb = k_blocks(mode, reduce) * (mode == kGrad ? 2 : 1);
-  const float round = mode == kGrad ? 0.25f : 0.21f, intake = mode == kGrad ? 125.f : 155.f;      // us, KB per us
+  const float round = mode == kGrad ? 0.24f : 0.16f, intake = mode == kGrad ? 142.f : 168.f;      // us, KB per us
   const int tiles_ch = (cols + 127) / 128;
   float best_t = 0.f;
   for (int tt = 16; tt <= 256 / nw; tt *= 2) {
@@ -108,8 +114,8 @@ static float plan_few(int mode, int rows, int cols, int reduce, FewPlan* best) {
     const int tiles_tok = (rows + tt - 1) / tt, ntok = rows < tt ? rows : tt;
     const long long tiles = (long long)tiles_ch * tiles_tok;
     if (tiles > 65536) continue;
-    const float l2 = (float)tiles * (float)nkb * (float)stage / 13.5e6f;
-    const float dram = (float)tiles_ch * (float)nkb * (float)(nw * 16384) / 5.6e6f;
+    const float l2 = (float)tiles * (float)nkb * (float)stage / (mode == kGrad ? 13.3e6f : 17.4e6f);
+    const float dram = (float)tiles_ch * (float)nkb * (float)(nw * 16384) / 6.8e6f;
     for (int i = 0; i < 6; ++i) {
       const int s = kSplits[i];
       if (s > nkb) break;
@@ -118,8 +124,8 @@ static float plan_few(int mode, int rows, int cols, int reduce, FewPlan* best) {
       const float live = (float)((tiles < resident ? (int)tiles : resident) * s);
       const float share = two && live > (float)kSMs ? live / (float)kSMs : 1.f;                   // CTAs that an SM feeds
       const float chain = (float)(waves * ((nkb + s - 1) / s)) * fmaxf(round, share * (float)stage / 1024.f / intake);
-      const float finish = 0.02f * (float)(nw * ntok) / (float)s + (s > 1 ? 2.0f + 0.022f * (float)(nw * ntok) : 0.f);
-      const float t = 2.5f + fmaxf(chain, fmaxf(l2, dram)) + finish + (float)(waves - 1) * (2.5f + finish);
+      const float finish = 0.02f * (float)(nw * ntok) / (float)s + (s > 1 ? 2.0f + 0.021f * (float)(nw * ntok) : 0.f);
+      const float t = 2.6f + overlapped(chain, l2, dram) + finish + (float)(waves - 1) * (2.5f + finish);
       if (best_t == 0.f || t < best_t) {
         const int stages = two ? half : full;
         best_t = t;
@@ -136,12 +142,12 @@ static long long set_width(PairJob* j, bool gated, int bn) {
   j->tiles_c = (j->cols + (gated ? bn : 2 * bn) - 1) / (gated ? bn : 2 * bn);
   return (long long)j->tiles_r * j->tiles_c * j->batches;
 }
-// Widths of the tiles of a launch on CTA pairs, and how the pairs share two lists of them.  MN-major k-blocks take as long whatever the
-// width (four loads of 64 x 64).  With one turn over both lists, whatever a pair had of the first, 12158 tokens of 768 x 1472 took
+// Widths of the tiles of a launch on CTA pairs, and how the pairs share two lists of them.  MN-major k-blocks of narrow tiles take
+// nearly as long as of wide ones (four loads of 64 x 64).  With one turn over both lists, whatever a pair had of the first, 12158 tokens of 768 x 1472 took
 // 116 us for what sharing does in 83.
 static float plan_pairs(int mode, PairPlan* plan) {
   static const int kWidth[3] = {128, 96, 64};
-  static const float kBlock[2][3] = {{0.32f, 0.25f, 0.205f}, {0.305f, 0.295f, 0.29f}};
+  static const float kBlock[2][3] = {{0.276f, 0.207f, 0.166f}, {0.27f, 0.235f, 0.20f}};
   const bool gated = is_gated(mode);
   PairPlan best = *plan;
   float best_t = 0.f;
@@ -153,8 +159,8 @@ static float plan_pairs(int mode, PairPlan* plan) {
       PairJob& j = plan->job[i];
       const int bn = kWidth[width[i]], nkb = k_blocks(mode, j.reduce) * (mode == kGrad && j.kind == 0 ? 2 : 1);
       tiles[i] = set_width(&j, gated, bn);
-      last[i] = 1.15f * (float)bn / 128.f;
-      each[i] = 1.5f + fmaxf((float)nkb * kBlock[mode == kGrad][width[i]], last[i]);
+      last[i] = 1.3f * (float)bn / 128.f;
+      each[i] = 1.f + fmaxf((float)nkb * kBlock[mode == kGrad][width[i]], last[i]);
       l2 += (float)tiles[i] * (float)nkb * (float)(32768 + 2 * bn * 128);
       dram += (float)nkb * 128.f * ((float)j.tiles_r * 256.f + (float)j.tiles_c * (float)(2 * bn)) * (float)j.batches;
     }
@@ -174,7 +180,7 @@ static float plan_pairs(int mode, PairPlan* plan) {
         if (longest == 0.f || fmaxf(a, b) < longest) { longest = fmaxf(a, b); share = s; }
       }
     }
-    const float t = 2.5f + fmaxf(longest, fmaxf(l2 / 12.5e6f, dram / 4.2e6f));
+    const float t = 3.f + overlapped(longest, l2 / 17e6f, dram / (mode == kGrad ? 3.2e6f : 6.3e6f));
     if (best_t == 0.f || t < best_t) {
       best_t = t;
       best = *plan;
