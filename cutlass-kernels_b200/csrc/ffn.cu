@@ -316,8 +316,12 @@ static int run_product(const ProductCall& c, cudaStream_t stream) {
   return too_many_tiles(plan.pair) ? CFK_ERR_UNSUPPORTED : run_pairs<MODE>(c, plan.pair, stream);
 }
 
+constexpr int kMaxSize = 0x7fffff00;
 static bool is16(int dt) { return dt == CFK_FP16 || dt == CFK_BF16; }
 static bool floats_ok(const float* p) { return p != nullptr && ((uintptr_t)p & 3u) == 0; }
+
+// Sizes that can be rounded up to a tile in 32 bits
+static bool size_ok(int m, int n, int k) { return m <= kMaxSize && n <= kMaxSize && k <= kMaxSize; }
 
 // 32-bit sums of 8-bit products: k * 128 * 128 stays below 2^31
 constexpr int kMaxI8Reduction = 131071;
@@ -332,7 +336,7 @@ static int check_gemm_i8(const cfk_gemm_i8_args* a, ProductCall* c) {
   c->y[0] = {a->b, CFK_INT8, a->n, a->k, packed(a->b_stride, a->k)};
   c->d[0] = {a->c, a->out_dtype, a->m, a->n, packed(a->c_stride, a->n)};
   if (!rows_ok(c->x[0]) || !rows_ok(c->y[0]) || !rows_ok(c->d[0])) return CFK_ERR_INVALID_ARG;
-  if (a->k > kMaxI8Reduction) return CFK_ERR_UNSUPPORTED;
+  if (a->k > kMaxI8Reduction || !size_ok(a->m, a->n, a->k)) return CFK_ERR_UNSUPPORTED;
   c->p.rows = a->m; c->p.cols = a->n; c->p.reduce = a->k;
   c->p.out = a->out_dtype;
   c->p.row_scale = a->a_scale; c->p.col_scale = a->b_scale; c->p.bias = a->bias;
@@ -361,7 +365,7 @@ static int check_gated(const cfk_ffn_gated_args* a, ProductCall* c) {
     if (a->gate == a->up || a->gate == a->h || a->up == a->h) return CFK_ERR_INVALID_ARG;
   }
   if (!rows_ok(c->x[0]) || !rows_ok(c->y[0]) || !rows_ok(c->y[1]) || !rows_ok(c->d[0])) return CFK_ERR_INVALID_ARG;
-  if (i8 && a->k > kMaxI8Reduction) return CFK_ERR_UNSUPPORTED;
+  if ((i8 && a->k > kMaxI8Reduction) || !size_ok(a->m, a->n, a->k)) return CFK_ERR_UNSUPPORTED;
   c->p.rows = a->m; c->p.cols = a->n; c->p.reduce = a->k;
   c->p.bf16 = a->dtype == CFK_BF16; c->p.out = a->out_dtype;
   c->p.act = a->activation; c->p.keep = a->gate != nullptr;
@@ -394,7 +398,7 @@ static int check_backward(const cfk_ffn_gated_backward_args* a, ProductCall* c) 
   // the only buffers that may be shared: dgate on gate, dup on up, row for row
   if (a->dgate == a->dup || a->dgate == a->up || a->dup == a->gate || a->dgate == a->dh || a->dup == a->dh) return CFK_ERR_INVALID_ARG;
   if ((a->dgate == a->gate || a->dup == a->up) && pre_s != dpre_s) return CFK_ERR_INVALID_ARG;
-  if ((long long)a->m * ((a->n + 7) / 8) > 0xffffff00LL) return CFK_ERR_UNSUPPORTED;
+  if (!size_ok(a->m, a->n, a->k) || (long long)a->m * ((a->n + 7) / 8) > 0xffffff00LL) return CFK_ERR_UNSUPPORTED;
   c->p.rows = a->m; c->p.cols = a->k; c->p.reduce = a->n;
   c->p.bf16 = dt == CFK_BF16; c->p.out = dt;
   return CFK_OK;

@@ -138,7 +138,7 @@ static cudaError_t launch_quantize(const void* src, int64_t ss, void* dst, int64
               : cols <= 4096 ? quantize_rows_kernel<SDT, 128, 4>
               : cols <= 8192 ? quantize_rows_kernel<SDT, 256, 4> : quantize_rows_kernel<SDT, 256, 8>;
   const int per = cols <= 1024 ? 8 : cols <= 2048 ? 4 : cols <= 4096 ? 2 : 1;    // rows per block
-  return launch_overlapped(kern, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, st, src, ss, (int8_t*)dst, ds, scale, rows,
+  return launch_overlapped(kern, dim3((unsigned)(((int64_t)rows + per - 1) / per)), dim3(256), 0, st, src, ss, (int8_t*)dst, ds, scale, rows,
                            cols);
 }
 

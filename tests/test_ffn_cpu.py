@@ -37,7 +37,8 @@ def test_quantize_refuses(lib, over, code):
     (dict(a_scale=0x4002), 1), (dict(bias=0x6001), 1), (dict(m=0), 1), (dict(n=-1), 1), (dict(k=0), 1),
     (dict(out_dtype=cfk.E4M3), 1), (dict(out_dtype=cfk.INT8), 1), (dict(a=0x1004), 1), (dict(c=0x3008), 1),
     (dict(k=72), 1), (dict(n=100), 1), (dict(n=100, c_stride=100), 1), (dict(a_stride=32), 1), (dict(b_stride=72), 1),
-    (dict(k=131072), 2), (dict(c_stride=1 << 31), 1),
+    (dict(k=131072), 2), (dict(c_stride=1 << 31), 1), (dict(m=0x7fffff01), 2),
+    (dict(m=0x7fffff00, n=0x7fffff00, c_stride=0x7fffffc0), 2),
 ])
 def test_gemm_i8_refuses(lib, over, code):
     kw = dict(a=0x1000, b=0x2000, c=0x3000, a_scale=0x4000, b_scale=0x5000, m=4, n=64, k=64, out_dtype=cfk.FP16)
@@ -53,7 +54,7 @@ def test_gemm_i8_refuses(lib, over, code):
     (dict(x_scale=0x6000), 1), (dict(dtype=cfk.INT8), 1), (dict(dtype=cfk.INT8, x_scale=0x6000, gate_scale=0x7000), 1),
     (dict(x=0x1002), 1), (dict(w_gate=0x2008), 1), (dict(k=60), 1), (dict(x_stride=60, k=60), 1), (dict(n=60), 1),
     (dict(gate=0x5000, up=0x6008), 1), (dict(gate=0x5000, up=0x5000), 1), (dict(gate=0x4000, up=0x5000), 1), (dict(gate=0x5000, up=0x6000, pre_stride=32), 1), (dict(h_stride=56), 1),
-    (dict(dtype=cfk.INT8, x_scale=0x6000, gate_scale=0x7000, up_scale=0x8000, k=131072), 2),
+    (dict(dtype=cfk.INT8, x_scale=0x6000, gate_scale=0x7000, up_scale=0x8000, k=131072), 2), (dict(m=0x7fffff01), 2),
 ])
 def test_ffn_gated_refuses(lib, over, code):
     kw = dict(x=0x1000, w_gate=0x2000, w_up=0x3000, h=0x4000, dtype=cfk.BF16, out_dtype=cfk.BF16, activation=0, m=4, n=64, k=64)
@@ -71,7 +72,7 @@ def test_ffn_gated_refuses(lib, over, code):
     (dict(dgate=0x1000), 1), (dict(dup=0x1000), 1),       # on dh
     (dict(dgate=0x5000, dpre_stride=128), 1),             # in place, other stride
     (dict(n=60), 1), (dict(dx=0x9000, dx_stride=32), 1), (dict(w_stride=68), 1),
-    (dict(m=1 << 30, n=256), 2),
+    (dict(m=1 << 30, n=256), 2), (dict(m=0x7fffffff), 2),
 ])
 def test_ffn_gated_backward_refuses(lib, over, code):
     kw = dict(dh=0x1000, x=0x2000, w_gate=0x3000, w_up=0x4000, gate=0x5000, up=0x6000, dgate=0x7000, dup=0x8000, dtype=cfk.BF16,

@@ -570,3 +570,62 @@ def test_offsets_beyond_32_bits(lib, cuda):
     lib.check_device()
     want = (x.double() @ b.double().T) * sx.double()[:, None] * sb.double()
     check(c, want, 2.0 ** -22 * want.abs())
+
+
+@pytest.mark.parametrize("m", [5, 300])
+def test_rows_that_lie_far_apart(lib, cuda, m):
+    """Forward with pre-activations and backward, in place, on matrices whose last rows begin behind 2^31 elements."""
+    n, k, dt = 72, 40, torch.float16
+    stride = ((1 << 31) // m + 4096) // 16 * 16
+    far = lambda: torch.empty(m * stride, dtype=dt, device="cuda").view(m, stride)[:, :n]      # noqa: E731
+    g = gen(m)
+    x, dh, h, gate, up = far(), far(), far(), far(), far()
+    x = x[:, :k]
+    x.copy_(randn(g, m, k)), dh.copy_(randn(g, m, n))
+    dx = far()[:, :k]
+    wg, wu = (randn(g, n, k) / 6).to(dt), (randn(g, n, k) / 6).to(dt)
+    dwg, dwu = torch.zeros_like(wg), torch.zeros_like(wu)
+    kw = dict(dtype=cfk.FP16, activation=cfk.ACT_SILU, m=m, n=n, k=k, x_stride=stride, pre_stride=stride)
+    lib.ffn_gated(x, wg, wu, h, out_dtype=cfk.FP16, gate=gate, up=up, h_stride=stride, **kw)
+    lib.check_device()
+    z, u = x.double() @ wg.double().T, x.double() @ wu.double().T
+    e = k * 2.0 ** -23 * (x.double().abs() @ wg.double().abs().T), k * 2.0 ** -23 * (x.double().abs() @ wu.double().abs().T)
+    check(h, activation64(cfk.ACT_SILU, z)[0] * u, gated_bound(cfk.ACT_SILU, z, u, *e, cfk.FP16))
+    gate0, up0 = gate.double(), up.double()
+    lib.ffn_gated_backward(dh, x, wg, wu, gate, up, gate, up, dx=dx, dw_gate=dwg, dw_up=dwu, dh_stride=stride, dpre_stride=stride,
+                           dx_stride=stride, **kw)
+    lib.check_device()
+    value, slope = activation64(cfk.ACT_SILU, gate0)
+    d = dh.double()
+    check(gate, d * up0 * slope, 3 * ACT_REL * (d * up0).abs() + half(cfk.FP16) * (d * up0 * slope).abs() + TINY[cfk.FP16])
+    dg, du, w = gate.double(), up.double(), (wg.double(), wu.double())
+    want = dg @ w[0] + du @ w[1]
+    b = 2 * n * 2.0 ** -23 * (dg.abs() @ w[0].abs() + du.abs() @ w[1].abs())
+    check(dx, want, b + half(cfk.FP16) * (want.abs() + b) + TINY[cfk.FP16])
+    want = du.T @ x.double()
+    b = m * 2.0 ** -23 * (du.abs().T @ x.double().abs())
+    check(dwu, want, b + half(cfk.FP16) * (want.abs() + b) + TINY[cfk.FP16])
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 256, 4096), (2, 256, 64), (2048, 2048, 256)])
+def test_products_skip_together_behind_a_wait_that_ran_out(lib, cuda, m, n, k):
+    """With the status word set the products write nothing; once it has been read the same calls run.  One token: clusters that
+    share a reduction; two: single CTAs; many: CTA pairs."""
+    outs, calls = block_calls(lib, m, n, k, 4)
+    xq, sx, c, dx, dwg, dwu = outs[6:]
+    calls(None)
+    lib.check_device()
+    want = [o.clone() for o in outs]
+    plan = lib.ffn_plan(cfk.FfnGatedArgs(cfk.FP16, cfk.FP16, 0, m, n, k, 16, 16, 16, 16, None, None, None, None, None, 0, 0, 0, 0))
+    assert (plan[0], plan[2] > 1) == {1: (1, True), 2: (1, False), 2048: (0, False)}[m]
+    products = [outs[0], outs[1], outs[2], outs[5], c, dx, dwg, dwu]
+    for o in products:
+        o.fill_(-3)
+    assert lib.selftest_wait_gives_up(20) == 0
+    calls(None)
+    rc, code = lib.device_status()
+    assert rc == 6 and code == 901
+    assert all(bool((o == -3).all()) for o in products)
+    calls(None)
+    lib.check_device()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
