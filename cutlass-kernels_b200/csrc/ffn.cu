@@ -444,6 +444,7 @@ extern "C" int cfk_ffn_gated_backward(const cfk_ffn_gated_backward_args* a, cfk_
   if (rc) return rc;
   const ProductPlan plan = plan_backward(a);
   if (too_many_tiles(plan.pair)) return CFK_ERR_UNSUPPORTED;
+  if (!device_status_block(&rc)) return rc;      // ahead of the first launch
   const cudaStream_t st = (cudaStream_t)stream;
   const cudaError_t e = a->dtype == CFK_FP16 ? launch_gate_grad<CFK_FP16>(a, st) : launch_gate_grad<CFK_BF16>(a, st);
   if (note_cuda(e, "gate gradient launch") != cudaSuccess) return CFK_ERR_LAUNCH;

@@ -230,7 +230,7 @@ int cfk_ffn_gated(const cfk_ffn_gated_args* args, cfk_stream_t stream);
  *   dx = dgate Wg + dup Wu,  dw_gate = dgate^T x,  dw_up = dup^T x.
  * dgate and dup are outputs that the products read: they are rounded to dtype, as the tensor core takes them, which adds to
  * each product an error of the size of its own rounding.  dgate may be the buffer of gate (or dup that of up) with the same
- * stride, which saves their memory.  Three launches; dx null leaves its product out, dw_gate and dw_up (both or neither) theirs.
+ * stride, which saves their memory.  Two or three launches; dx null leaves its product out, dw_gate and dw_up (both or neither) theirs.
  * act'(0) of RELU is 0.
  */
 typedef struct cfk_ffn_gated_backward_args {
