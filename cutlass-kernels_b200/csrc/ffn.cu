@@ -143,8 +143,8 @@ static long long set_width(PairJob* j, bool gated, int bn) {
   return (long long)j->tiles_r * j->tiles_c * j->batches;
 }
 // Widths of the tiles of a launch on CTA pairs, and how the pairs share two lists of them.  MN-major k-blocks of narrow tiles take
-// nearly as long as of wide ones (four loads of 64 x 64).  With one turn over both lists, whatever a pair had of the first, 12158 tokens of 768 x 1472 took
-// 116 us for what sharing does in 83.
+// nearly as long as of wide ones (four loads of 64 x 64).  The gradients of 12158 tokens of 768 x 1472 take 108 us; with the second list
+// dealt to all pairs alike, whatever they had of the first, 171.
 static float plan_pairs(int mode, PairPlan* plan) {
   static const int kWidth[3] = {128, 96, 64};
   static const float kBlock[2][3] = {{0.276f, 0.207f, 0.166f}, {0.27f, 0.235f, 0.20f}};

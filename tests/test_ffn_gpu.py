@@ -380,6 +380,28 @@ def test_every_cut_of_the_backward_pass(lib, cuda):
         run_backward(lib, cfk.FP16 if i % 2 else cfk.BF16, ACTS[i % 4], m, n, k, seed=i)
 
 
+@pytest.mark.parametrize("seed", range(4))
+def test_random_calls(lib, cuda, seed):
+    """Sizes over the whole range, on a logarithm, with types, padding, options and gradients left out at random."""
+    rng = random.Random(100 + seed)
+    log = lambda lo, hi: int(round(lo * (hi / lo) ** rng.random()))      # noqa: E731
+    for i in range(25):
+        m, n, k, pad = log(1, 2500), log(1, 3000), log(1, 3000), rng.choice([0, 0, 1, 3])
+        if rng.random() < 0.5:
+            n, k = max(64, n // 64 * 64), max(64, k // 64 * 64)
+        out, act = rng.choice([cfk.FP16, cfk.BF16]), rng.choice(ACTS)
+        kind = rng.randrange(4)
+        if kind == 0:
+            run_gemm_i8(lib, m, n, k, rng.choice([cfk.FP16, cfk.BF16, cfk.FP32]), bias=rng.random() < 0.5, pad=pad, seed=i)
+        elif kind == 1:
+            run_gated(lib, out, out, act, m, n, k, keep=rng.random() < 0.5, pad=pad, seed=i)
+        elif kind == 2:
+            run_gated(lib, cfk.INT8, out, act, m, n, k, keep=rng.random() < 0.5, pad=pad, seed=i)
+        else:
+            parts = rng.choice([(True, True), (True, True), (True, False), (False, True)])
+            run_backward(lib, out, act, m, n, k, pad=pad, seed=i, in_place=rng.random() < 0.5, dx=parts[0], dw=parts[1])
+
+
 # ---- together ------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("m", [1, 19, 300])
 def test_an_8_bit_block_end_to_end(lib, cuda, m):
