@@ -90,9 +90,9 @@ static int k_blocks(int mode, int reduce) {
 }
 
 // Three things that run beside each other take the longest one's time and some of the others'.
-static float overlapped(float a, float b, float c) {
+static float overlapped(float a, float b, float c, float beside) {
   const float most = fmaxf(a, fmaxf(b, c));
-  return most + 0.22f * (a + b + c - most);
+  return most + beside * (a + b + c - most);
 }
 
 // Clusters of 1, 2, 3, 4, 6 and 8 CTAs that are resident at once, with one and with two CTAs per SM, as
@@ -100,12 +100,18 @@ static float overlapped(float a, float b, float c) {
 constexpr int kSplits[6] = {1, 2, 3, 4, 6, 8};
 constexpr int kResident[2][6] = {{148, 74, 45, 33, 22, 15}, {296, 148, 93, 71, 45, 33}};
 
-// The kernel for few tokens: the longest of what a CTA takes for its k-blocks (a round of the ring, or what an SM takes in), the
-// tiles' traffic from L2 and the weights' from DRAM; then the epilogue and the exchange of a split.  One CTA per SM with the deepest
-// ring where the clusters fit that way: one gated token of 11264 x 4096 bf16 32.0 us against 36.2 with half of it.
+// The kernel for few tokens: what a CTA takes for its k-blocks (a round of the ring, or what an SM takes in), the tiles' traffic from L2 and
+// the weights' from DRAM run beside each other; then the epilogue, the exchange of a split, and a start that grows with the CTAs
+// where two share an SM.  One CTA per SM with the deepest ring where the clusters fit that way: one gated token of 11264 x 4096 bf16
+// 32.0 us against 36.2 with half of it.
+struct FewCost {
+  float start, crowd, round, intake, l2, dram, beside, column, exchange, per_column, per_part, wave;   // us; KB and bytes per us
+};
 static float plan_few(int mode, int rows, int cols, int reduce, FewPlan* best) {
+  static const FewCost kCost[2] = {{2.5f, 0.33f, 0.166f, 167.f, 18.3e6f, 6.95e6f, 0.23f, 0.02f, 1.8f, 0.023f, 0.045f, 1.7f},
+                                   {2.5f, 0.8f, 0.242f, 149.f, 15.9e6f, 8e6f, 0.4f, 0.012f, 0.8f, 0.023f, 0.135f, 0.8f}};
+  const FewCost& c = kCost[mode == kGrad];
   const int nw = few_weights(mode), nkb = k_blocks(mode, reduce) * (mode == kGrad ? 2 : 1);
-  const float round = mode == kGrad ? 0.24f : 0.16f, intake = mode == kGrad ? 142.f : 168.f;      // us, KB per us
   const int tiles_ch = (cols + 127) / 128;
   float best_t = 0.f;
   for (int tt = 16; tt <= 256 / nw; tt *= 2) {
@@ -114,18 +120,20 @@ static float plan_few(int mode, int rows, int cols, int reduce, FewPlan* best) {
     const int tiles_tok = (rows + tt - 1) / tt, ntok = rows < tt ? rows : tt;
     const long long tiles = (long long)tiles_ch * tiles_tok;
     if (tiles > 65536) continue;
-    const float l2 = (float)tiles * (float)nkb * (float)stage / (mode == kGrad ? 13.3e6f : 17.4e6f);
-    const float dram = (float)tiles_ch * (float)nkb * (float)(nw * 16384) / 6.8e6f;
+    const float l2 = (float)tiles * (float)nkb * (float)stage / c.l2;
+    const float dram = (float)tiles_ch * (float)nkb * (float)(nw * 16384) / c.dram;
     for (int i = 0; i < 6; ++i) {
       const int s = kSplits[i];
       if (s > nkb) break;
       const bool two = half >= 3 && tiles > kResident[0][i];
       const int resident = kResident[two][i], waves = (int)((tiles + resident - 1) / resident);
-      const float live = (float)((tiles < resident ? (int)tiles : resident) * s);
-      const float share = two && live > (float)kSMs ? live / (float)kSMs : 1.f;                   // CTAs that an SM feeds
-      const float chain = (float)(waves * ((nkb + s - 1) / s)) * fmaxf(round, share * (float)stage / 1024.f / intake);
-      const float finish = 0.02f * (float)(nw * ntok) / (float)s + (s > 1 ? 2.0f + 0.021f * (float)(nw * ntok) : 0.f);
-      const float t = 2.6f + overlapped(chain, l2, dram) + finish + (float)(waves - 1) * (2.5f + finish);
+      const float live = (float)((tiles < resident ? (int)tiles : resident) * s) / (float)kSMs;     // CTAs per SM
+      const float chain = (float)(waves * ((nkb + s - 1) / s)) *
+                          fmaxf(c.round, (two && live > 1.f ? live : 1.f) * (float)stage / 1024.f / c.intake);
+      const float finish = c.column * (float)(nw * ntok) / (float)s +
+                           (s > 1 ? c.exchange + c.per_column * (float)(nw * ntok) + c.per_part * (float)s : 0.f);
+      const float t = c.start + (two ? c.crowd * live : 0.f) + overlapped(chain, l2, dram, c.beside) + finish +
+                      (float)(waves - 1) * (c.wave + finish);
       if (best_t == 0.f || t < best_t) {
         const int stages = two ? half : full;
         best_t = t;
@@ -180,7 +188,7 @@ static float plan_pairs(int mode, PairPlan* plan) {
         if (longest == 0.f || fmaxf(a, b) < longest) { longest = fmaxf(a, b); share = s; }
       }
     }
-    const float t = 3.f + overlapped(longest, l2 / 17e6f, dram / (mode == kGrad ? 3.2e6f : 6.3e6f));
+    const float t = 3.f + overlapped(longest, l2 / 17e6f, dram / (mode == kGrad ? 3.2e6f : 6.3e6f), 0.22f);
     if (best_t == 0.f || t < best_t) {
       best_t = t;
       best = *plan;
