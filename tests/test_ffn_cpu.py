@@ -84,6 +84,7 @@ def test_ffn_gated_backward_refuses(lib, over, code):
 
 
 P = list(range(0x1000, 0x10000, 0x1000))
+TOKENS = [16, 32, 48, 64, 96, 128, 192, 256]
 
 
 def product(m, n, k, out=cfk.BF16):
@@ -112,7 +113,7 @@ def test_plans_can_be_run_and_cover_both_kernels(lib):
             few, width, parts = plan = lib.ffn_plan(args)
             seen.add((widest, few))
             if few:
-                assert width in (16, 32, 64, 128, 256) and width <= widest and (width == 16 or width < 2 * m)
+                assert width in TOKENS and width <= widest and (width == 16 or TOKENS[TOKENS.index(width) - 1] < m)
                 assert parts in (1, 2, 3, 4, 6, 8)
             else:
                 assert width in (64, 96, 128) and parts == 1
@@ -122,7 +123,7 @@ def test_plans_can_be_run_and_cover_both_kernels(lib):
                 assert not few
         assert lib.ffn_plan(product(m, n, k, cfk.FP32)) == lib.ffn_plan(product(m, n, k))
         few, width, parts, dw = lib.ffn_plan(backward(m, n, k))
-        assert (width in (16, 32, 64, 128, 256) and parts in (1, 2, 3, 4, 6, 8)) if few else (width in (64, 96, 128) and parts == 1)
+        assert (width in TOKENS and parts in (1, 2, 3, 4, 6, 8)) if few else (width in (64, 96, 128) and parts == 1)
         assert dw in (64, 96, 128)
         assert lib.ffn_plan(backward(m, n, k, dx=False))[:3] == (0, 0, 1) and lib.ffn_plan(backward(m, n, k, dw=False))[3] == 0
     assert seen == {(256, 0), (256, 1), (128, 0), (128, 1)}
