@@ -101,10 +101,10 @@ static float overlapped(float a, float b, float c, float beside) {
 constexpr int kSplits[6] = {1, 2, 3, 4, 6, 8};
 constexpr int kResident[2][6] = {{148, 74, 45, 33, 22, 15}, {296, 148, 93, 71, 45, 33}};
 
-// The kernel for few tokens: what a CTA takes for its k-blocks (a round of the ring, or what an SM takes in), the tiles' traffic from L2 and
-// the weights' from DRAM run beside each other; then the epilogue, the exchange of a split, and a start that grows with the CTAs
-// where two share an SM.  One CTA per SM with the deepest ring where the clusters fit that way: one gated token of 11264 x 4096 bf16
-// 32.0 us against 36.2 with half of it.
+// The kernel for few tokens: what a CTA takes for its k-blocks (a round of the ring, or what an SM takes in), the tiles' traffic
+// from L2 and the weights' from DRAM run beside each other; then the epilogue, the exchange of a split, and a start that grows with
+// the CTAs where two share an SM.  One CTA per SM with the deepest ring where the clusters fit that way: one gated token of
+// 11264 x 4096 bf16 32.0 us against 36.2 with half of it.
 struct FewCost {
   float start, crowd, round, intake, l2, dram, beside, column, exchange, per_column, per_part, wave;   // us; KB and bytes per us
 };

@@ -177,9 +177,10 @@ few_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_consta
         const uint64_t a0 = make_smem_desc(at + w * C::WB, W_MN ? C::WB / 2 : 16, 1024, kSwizzle128B);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
-          const uint32_t acc = kb != kb0 || kk != 0 ? 1u : 0u;
-          if constexpr (I8) umma_ss_i8<false>(tmem_base + w * acc_cols, desc_advance(a0, kk * WSTEP), desc_advance(b0, kk * 32), idesc, acc, leader);
-          else umma_ss_e<false, false>(tmem_base + w * acc_cols, desc_advance(a0, kk * WSTEP), desc_advance(b0, kk * 32), idesc, acc, leader);
+          const uint32_t acc = kb != kb0 || kk != 0 ? 1u : 0u, d = tmem_base + w * acc_cols;
+          const uint64_t a = desc_advance(a0, kk * WSTEP), b = desc_advance(b0, kk * 32);
+          if constexpr (I8) umma_ss_i8<false>(d, a, b, idesc, acc, leader);
+          else umma_ss_e<false, false>(d, a, b, idesc, acc, leader);
         }
       }
       umma_commit_e<false>(bar_empty + 8 * s, leader);

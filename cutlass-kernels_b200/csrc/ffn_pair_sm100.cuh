@@ -11,17 +11,17 @@
 //                operand is contiguous: both are MN-major.
 //
 // Roles, ring and tensor-memory double buffer are those of gemm_kernel: warp 0 TMA, warp 1 of the leader UMMA (cta_group::2); but
-// two groups of four epilogue warps, which write with ordinary stores.  (A TMA store writes whole 16-byte pieces, so behind the last element
-// of a row it would put zeros up to the next multiple of 16 bytes; and the hand-over of staging tiles between four warps and a
-// storing thread took 0.6 us per 32 columns, most of a tile whose reduction is short.)
+// two groups of four epilogue warps, which write with ordinary stores.  (A TMA store writes whole 16-byte pieces, so behind the
+// last element of a row it would put zeros up to the next multiple of 16 bytes; and the hand-over of staging tiles between four
+// warps and a storing thread took 0.6 us per 32 columns, most of a tile whose reduction is short.)
 // An MN-major operand lands as spans of 64 columns, [span][64 k-rows][128 bytes], each with the 128-byte swizzle; what lies
 // behind a matrix is zero-filled in both operands, so ragged reductions need no mask.
 //
 // A tile is 2 bn accumulator columns wide, bn = 128, 96 or 64 by what fills the last wave of pairs best (ffn.cu).  Bound by the tensor
 // core: 512 clk of MMA per k-block of 128 bytes at bn = 128 against 32 KB of loads per SM and, in the gated modes, an epilogue of
 // two special-function operations per element of h that runs beside the next tile's main loop.  The pipe is 88 to 96 % active, at
-// the 1.3 GHz that the power cap leaves: gated 8192 x 11264 x 4096 in bf16 1051 us, 1440 TFLOP/s; its 8-bit form 507 us and 8192^3 in 8 bits
-// 370 us, 2980 TOP/s; the gradients of 8192 x 11264 x 4096 2300 to 2450 us, 1230 to 1310 TFLOP/s.
+// the 1.3 GHz that the power cap leaves: gated 8192 x 11264 x 4096 in bf16 1051 us, 1440 TFLOP/s; its 8-bit form 507 us and 8192^3
+// in 8 bits 370 us, 2980 TOP/s; the gradients of 8192 x 11264 x 4096 2300 to 2450 us, 1230 to 1310 TFLOP/s.
 #pragma once
 #include "common.cuh"
 #include "ffn_act.cuh"
@@ -94,11 +94,11 @@ __device__ __forceinline__ void store_columns(const ProductParams& p, int which,
   }
 }
 
-// Through shared memory of each epilogue warp, 32 rows x 128 bytes (64 columns): 8 threads per row, so that an instruction writes whole
-// lines and not a sector of 32 of them.  0.7 us per 64 columns of a tile instead of 0.9, at the price of a stage of the ring: taken for
-// gradients of the weights from up to 512 tokens, which are little but writes (5632 x 2048 from 64 tokens: 16.7 us against 18.1; 2048 x 4096 from
-// 300: 17.8 / 18.7; 2731 x 1027 from 777: 19.5 / 19.1); elsewhere the stage is worth more (8-bit products of 1500 x 4096 x 1024: 13.7
-// against 12.2).  The pieces of a row are exchanged by the row's index, against bank conflicts.
+// Through shared memory of each epilogue warp, 32 rows x 128 bytes (64 columns): 8 threads per row, so that an instruction writes
+// whole lines and not a sector of 32 of them.  0.7 us per 64 columns of a tile instead of 0.9, at the price of a stage of the ring:
+// taken for gradients of the weights from up to 512 tokens, which are little but writes (5632 x 2048 from 64 tokens: 16.7 us against
+// 18.1; 2048 x 4096 from 300: 17.8 / 18.7; 2731 x 1027 from 777: 19.5 / 19.1); elsewhere the stage is worth more (8-bit products of
+// 1500 x 4096 x 1024: 13.7 against 12.2).  The pieces of a row are exchanged by the row's index, against bank conflicts.
 __device__ __forceinline__ uint32_t staged_at(uint32_t tile, int r, int piece) { return tile + r * 128 + ((piece ^ (r & 7)) << 4); }
 __device__ __forceinline__ void stage_columns(uint32_t tile, int r, int piece0, bool bf16, const float (&v)[32]) {
 #pragma unroll

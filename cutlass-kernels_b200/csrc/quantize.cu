@@ -52,8 +52,8 @@ __device__ __noinline__ uint32_t quantize_by_division(float x, float scale) {   
 }
 
 template <int SDT, int G, int U>
-__global__ void __launch_bounds__(256, U > 4 ? 2 : elem_bytes(SDT) == 2 ? 5 : 4) quantize_rows_kernel(const void* src, int64_t src_stride, int8_t* dst,
-                                                            int64_t dst_stride, float* scale, int rows, int cols) {
+__global__ void __launch_bounds__(256, U > 4 ? 2 : elem_bytes(SDT) == 2 ? 5 : 4)
+quantize_rows_kernel(const void* src, int64_t src_stride, int8_t* dst, int64_t dst_stride, float* scale, int rows, int cols) {
   constexpr int PER = 256 / G, SB = elem_bytes(SDT), E = 16 / SB;   // elements per 16-byte access: 8, or 4 of fp32
   constexpr int NH = 8 / E;                                        // accesses per vector of 8
   using Half = ElemPack<SDT, E>;
@@ -150,8 +150,8 @@ static cudaError_t launch_quantize(const void* src, int64_t ss, void* dst, int64
               : cols <= 4096 ? quantize_rows_kernel<SDT, 128, 4>
               : cols <= 8192 ? quantize_rows_kernel<SDT, 256, 4> : quantize_rows_kernel<SDT, 256, 8>;
   const int per = cols <= 1024 ? 8 : cols <= 2048 ? 4 : cols <= 4096 ? 2 : 1;    // rows per block
-  return launch_overlapped(kern, dim3((unsigned)(((int64_t)rows + per - 1) / per)), dim3(256), 0, st, src, ss, (int8_t*)dst, ds, scale, rows,
-                           cols);
+  const unsigned blocks = (unsigned)(((int64_t)rows + per - 1) / per);
+  return launch_overlapped(kern, dim3(blocks), dim3(256), 0, st, src, ss, (int8_t*)dst, ds, scale, rows, cols);
 }
 
 }  // namespace cfk
