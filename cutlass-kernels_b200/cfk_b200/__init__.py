@@ -86,11 +86,12 @@ class FfnGatedBackwardArgs(C.Structure):
 
 
 def _ptr(x):
-    if x is None:
-        return None
-    if isinstance(x, int):
+    if x is None or x.__class__ is int:
         return x
-    return int(x.data_ptr())
+    try:
+        return x.data_ptr()
+    except AttributeError:       # an integer of another type
+        return int(x)
 
 
 _PACKED = (0, 0, 0)
