@@ -64,6 +64,23 @@ def test_quantize_ties_zero_rows_underflow_and_what_is_not_finite(lib, cuda):
     assert bool(scale[-9:].isnan().all()) and bool((q[-9:] == 0).all()) and scale[1] == 0
 
 
+def test_quantize_next_to_the_middle_between_two_integers(lib, cuda):
+    """Values two units in the last place or less from (k + 1/2) scale, for scales over the range of fp32: where a quotient that is
+    not rounded correctly would go to the wrong side."""
+    rows, cols = 512, 2048
+    g = gen(8)
+    amax = torch.exp2(torch.rand(rows, 1, generator=g, device="cuda") * 240 - 120)
+    middle = (torch.randint(-126, 126, (rows, cols), generator=g, device="cuda") + 0.5) * (amax / torch.full_like(amax, 127.0))
+    nudge = torch.randint(-2, 3, (rows, cols), generator=g, device="cuda", dtype=torch.int32)
+    x = (middle.view(torch.int32) + nudge).view(torch.float32)
+    x[:, :1] = amax
+    q, scale = torch.zeros(rows, cols, dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda")
+    lib.quantize_rows(x, q, scale, src_dtype=cfk.FP32, rows=rows, cols=cols)
+    lib.check_device()
+    want_q, want_scale = quantize_definition(x)
+    assert torch.equal(scale, want_scale) and torch.equal(q, want_q)
+
+
 # ---- 8-bit product -----------------------------------------------------------------------------------------------------------------
 def run_gemm_i8(lib, m, n, k, out, bias, pad=0, seed=0, stream=None):
     g = gen(seed)
