@@ -18,16 +18,19 @@ static int64_t packed(int64_t stride, int cols) { return stride == 0 ? cols : st
 // dgate = dh * up * act'(gate), dup = dh * act(gate).  Memory bound: three 16-bit values in, two out, 16 bytes per access, a thread
 // reads its elements of all three before it writes, so the results may take the place of gate and up.  8192 x 11264 bf16: 152 us,
 // 6.1 TB/s.
+// Behind a wait that gave up it writes nothing, as the products that follow it: in place it would take the inputs of a repeated call.
+// The status word is read beside the elements, so the test costs a barrier and not a memory latency.
 template <int DT, int ACT>
 __global__ void __launch_bounds__(256) gate_grad_kernel(const uint16_t* dh, const uint16_t* gate, const uint16_t* up, uint16_t* dgate,
                                                         uint16_t* dup, int64_t dh_stride, int64_t pre_stride,
-                                                        int64_t dpre_stride, int cols, uint32_t nvec, uint32_t total) {
+                                                        int64_t dpre_stride, int cols, uint32_t nvec, uint32_t total,
+                                                        const int* status) {
   grid_dependency_launch();
   grid_dependency_wait();
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
-  if (idx >= total) return;
-  const uint32_t row = idx / nvec;
-  const int col = (int)(idx - row * nvec) * 8;
+  const bool exists = idx < total;
+  const uint32_t row = exists ? idx / nvec : 0u;
+  const int col = exists ? (int)(idx - row * nvec) * 8 : cols;
   dh += row * dh_stride + col;
   gate += row * pre_stride + col;
   up += row * pre_stride + col;
@@ -48,6 +51,7 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const uint16_t* dh, cons
       u.h[i] = in ? up[i] : (uint16_t)0;
     }
   }
+  if (cta_should_skip(status)) return;
   float x[8], y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -68,14 +72,15 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const uint16_t* dh, cons
 }
 
 template <int DT>
-static cudaError_t launch_gate_grad(const cfk_ffn_gated_backward_args* a, cudaStream_t st) {
+static cudaError_t launch_gate_grad(const cfk_ffn_gated_backward_args* a, const int* status, cudaStream_t st) {
   const int64_t dh_s = packed(a->dh_stride, a->n), pre_s = packed(a->pre_stride, a->n), dpre_s = packed(a->dpre_stride, a->n);
   const uint32_t nvec = (uint32_t)((a->n + 7) / 8), total = (uint32_t)a->m * nvec;
   auto kern = a->activation == CFK_ACT_SILU ? gate_grad_kernel<DT, CFK_ACT_SILU>
               : a->activation == CFK_ACT_GELU ? gate_grad_kernel<DT, CFK_ACT_GELU>
               : a->activation == CFK_ACT_GELU_TANH ? gate_grad_kernel<DT, CFK_ACT_GELU_TANH> : gate_grad_kernel<DT, CFK_ACT_RELU>;
   return launch_overlapped(kern, dim3((total + 255u) / 256u), dim3(256), 0, st, (const uint16_t*)a->dh, (const uint16_t*)a->gate,
-                           (const uint16_t*)a->up, (uint16_t*)a->dgate, (uint16_t*)a->dup, dh_s, pre_s, dpre_s, a->n, nvec, total);
+                           (const uint16_t*)a->up, (uint16_t*)a->dgate, (uint16_t*)a->dup, dh_s, pre_s, dpre_s, a->n, nvec, total,
+                           status);
 }
 
 // ---- cuts -------------------------------------------------------------------------------------------------------------------
@@ -283,21 +288,25 @@ static int prepare_results(const ProductCall& c, ProductParams* p) {
   return rc;
 }
 
+// All that can fail ahead of a launch: a call of several launches prepares every one before the first.
+struct FewLaunch { ProductMaps maps; ProductParams p; FewPlan plan; };
+struct PairLaunch { ProductMaps maps; ProductParams p; PairPlan plan; };
+
 template <int MODE>
-static int run_few(const ProductCall& c, const FewPlan& few, cudaStream_t stream) {
-  ProductParams p = c.p;
-  ProductMaps maps;
-  std::memset(&maps, 0, sizeof(maps));
-  int rc = prepare_results(c, &p);
+static int prepare_few(const ProductCall& c, const FewPlan& few, FewLaunch* l) {
+  l->p = c.p;
+  l->plan = few;
+  std::memset(&l->maps, 0, sizeof(l->maps));
+  int rc = prepare_results(c, &l->p);
   for (int i = 0; i < 2 && rc == CFK_OK; ++i) {
-    if (c.x[i].base) rc = encode(&maps.x[i], c.x[i], few.tt);
-    if (rc == CFK_OK && c.y[i].base) rc = encode(&maps.y[i], c.y[i], MODE == kGrad ? 64 : 128);
+    if (c.x[i].base) rc = encode(&l->maps.x[i], c.x[i], few.tt);
+    if (rc == CFK_OK && c.y[i].base) rc = encode(&l->maps.y[i], c.y[i], MODE == kGrad ? 64 : 128);
   }
-  return rc ? rc : launch_few_product<MODE>(maps, p, few, stream);
+  return rc ? rc : allow_few_product<MODE>();
 }
 
 template <int MODE>
-static int run_pairs(const ProductCall& c, PairPlan plan, cudaStream_t stream) {
+static int prepare_pairs(const ProductCall& c, PairPlan plan, PairLaunch* l) {
   const int first = plan.job[0].tiles_r * plan.job[0].tiles_c * plan.job[0].batches;
   plan.most = first / plan.pairs;
   plan.more = first % plan.pairs;
@@ -308,22 +317,29 @@ static int run_pairs(const ProductCall& c, PairPlan plan, cudaStream_t stream) {
     j.per_band = make_divisor((uint32_t)(kGemmBand * j.tiles_c));
     j.tail_rows = make_divisor((uint32_t)(j.tiles_r % kGemmBand ? j.tiles_r % kGemmBand : 1));
   }
-  ProductParams p = c.p;
-  ProductMaps maps;
-  std::memset(&maps, 0, sizeof(maps));
-  int rc = prepare_results(c, &p);
+  l->p = c.p;
+  l->plan = plan;
+  std::memset(&l->maps, 0, sizeof(l->maps));
+  int rc = prepare_results(c, &l->p);
   for (int i = 0; i < 2 && rc == CFK_OK; ++i)
-    if (c.x[i].base) rc = encode(&maps.x[i], c.x[i], MODE == kGrad ? 64 : 128);
+    if (c.x[i].base) rc = encode(&l->maps.x[i], c.x[i], MODE == kGrad ? 64 : 128);
   for (int i = 0; i < 3 && rc == CFK_OK; ++i)
-    if (c.y[i].base) rc = encode(&maps.y[i], c.y[i], MODE == kGrad ? 64 : plan.job[0].bn);
-  return rc ? rc : launch_pair_product<MODE>(maps, p, plan, stream);
+    if (c.y[i].base) rc = encode(&l->maps.y[i], c.y[i], MODE == kGrad ? 64 : plan.job[0].bn);
+  return rc ? rc : allow_pair_product<MODE>();
 }
 
 template <int MODE>
 static int run_product(const ProductCall& c, cudaStream_t stream) {
   const ProductPlan plan = plan_product(MODE, c.p.rows, c.p.cols, c.p.reduce);
-  if (plan.few.tt > 0) return run_few<MODE>(c, plan.few, stream);
-  return too_many_tiles(plan.pair) ? CFK_ERR_UNSUPPORTED : run_pairs<MODE>(c, plan.pair, stream);
+  if (plan.few.tt > 0) {
+    FewLaunch l;
+    const int rc = prepare_few<MODE>(c, plan.few, &l);
+    return rc ? rc : launch_few_product<MODE>(l.maps, l.p, l.plan, stream);
+  }
+  if (too_many_tiles(plan.pair)) return CFK_ERR_UNSUPPORTED;
+  PairLaunch l;
+  const int rc = prepare_pairs<MODE>(c, plan.pair, &l);
+  return rc ? rc : launch_pair_product<MODE>(l.maps, l.p, l.plan, stream);
 }
 
 constexpr int kMaxSize = 0x7fffff00;
@@ -454,12 +470,18 @@ extern "C" int cfk_ffn_gated_backward(const cfk_ffn_gated_backward_args* a, cfk_
   if (rc) return rc;
   const ProductPlan plan = plan_backward(a);
   if (too_many_tiles(plan.pair)) return CFK_ERR_UNSUPPORTED;
-  if (!device_status_block(&rc)) return rc;      // ahead of the first launch
+  const int* status = device_status_block(&rc);
+  if (!status) return rc;
+  // in place the first launch takes the place of its inputs: nothing that could fail is left for after it but the launches
+  FewLaunch few;
+  PairLaunch pair;
+  if (plan.few.tt > 0 && (rc = prepare_few<kGrad>(c, plan.few, &few))) return rc;
+  if (plan.pair.jobs > 0 && (rc = prepare_pairs<kGrad>(c, plan.pair, &pair))) return rc;
   const cudaStream_t st = (cudaStream_t)stream;
-  const cudaError_t e = a->dtype == CFK_FP16 ? launch_gate_grad<CFK_FP16>(a, st) : launch_gate_grad<CFK_BF16>(a, st);
+  const cudaError_t e = a->dtype == CFK_FP16 ? launch_gate_grad<CFK_FP16>(a, status, st) : launch_gate_grad<CFK_BF16>(a, status, st);
   if (note_cuda(e, "gate gradient launch") != cudaSuccess) return CFK_ERR_LAUNCH;
-  if (plan.few.tt > 0 && (rc = run_few<kGrad>(c, plan.few, st))) return rc;
-  return plan.pair.jobs > 0 ? run_pairs<kGrad>(c, plan.pair, st) : CFK_OK;
+  if (plan.few.tt > 0 && (rc = launch_few_product<kGrad>(few.maps, few.p, few.plan, st))) return rc;
+  return plan.pair.jobs > 0 ? launch_pair_product<kGrad>(pair.maps, pair.p, pair.plan, st) : CFK_OK;
 }
 extern "C" int cfk_ffn_gated_backward_plan(const cfk_ffn_gated_backward_args* a, int plan[4]) {
   ProductCall c;

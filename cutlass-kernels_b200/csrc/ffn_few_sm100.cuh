@@ -318,9 +318,9 @@ few_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_consta
 }
 
 template <int MODE>
+int allow_few_product() { return allow_shared_memory(few_product_kernel<MODE>, kFewSmemFull); }
+template <int MODE>
 int launch_few_product(const ProductMaps& maps, const ProductParams& p, const FewPlan& f, cudaStream_t stream) {
-  const int rc = allow_shared_memory(few_product_kernel<MODE>, kFewSmemFull);
-  if (rc) return rc;
   const dim3 grid((unsigned)(f.tiles_ch * f.tiles_tok * f.splits));
   const size_t smem = kFewHead + (size_t)f.stages * (few_weights(MODE) * FewCfg::WB + f.tt * 128);
   return note_cuda(launch_overlapped_in(f.splits, few_product_kernel<MODE>, grid, dim3(FewCfg::NTHREADS), smem, stream, maps, p, f),

@@ -1,4 +1,5 @@
 #include "ffn_pair_sm100.cuh"
 namespace cfk {
+template int allow_pair_product<kGatedI8>();
 template int launch_pair_product<kGatedI8>(const ProductMaps&, const ProductParams&, PairPlan, cudaStream_t);
 }

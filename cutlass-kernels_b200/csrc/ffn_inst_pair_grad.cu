@@ -1,4 +1,5 @@
 #include "ffn_pair_sm100.cuh"
 namespace cfk {
+template int allow_pair_product<kGrad>();
 template int launch_pair_product<kGrad>(const ProductMaps&, const ProductParams&, PairPlan, cudaStream_t);
 }

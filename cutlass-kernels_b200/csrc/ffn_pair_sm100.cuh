@@ -40,6 +40,7 @@ struct PairCfg {
   static constexpr int HEADB = 1024 + 256, MAXSTAGE = 8;           // alignment slack and the barrier block
   static constexpr int STAGEB = 32 * 128;                          // output staging of an epilogue warp, where results are staged
   static constexpr int NTHREADS = 64 + GROUPS * 128;
+  static constexpr int SMEM = 227 * 1024 - 128;                    // and a few static bytes of the kernel
   static_assert(8 * (2 * MAXSTAGE + 4) + 8 <= 256, "barrier block overflows");
 };
 
@@ -402,17 +403,16 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
 }
 
 template <int MODE>
+int allow_pair_product() { return allow_shared_memory(pair_product_kernel<MODE>, PairCfg::SMEM); }
+template <int MODE>
 int launch_pair_product(const ProductMaps& maps, const ProductParams& p, PairPlan plan, cudaStream_t stream) {
   using C = PairCfg;
-  constexpr int SMEM = 227 * 1024 - 128;                  // and a few static bytes of the kernel
-  const int rc = allow_shared_memory(pair_product_kernel<MODE>, SMEM);
-  if (rc) return rc;
   // narrower tiles leave room for more stages
   int bn = plan.job[0].bn;
   if (plan.jobs > 1 && plan.job[1].bn > bn) bn = plan.job[1].bn;
   plan.y_bytes = MODE == kGrad ? (bn > 64 ? 2 : 1) * C::SPANB : bn * 128;
   const int head = C::HEADB + (MODE == kGrad && plan.staged ? 4 * C::GROUPS * C::STAGEB : 0);
-  plan.stages = (SMEM - head) / (C::XB + plan.y_bytes);
+  plan.stages = (C::SMEM - head) / (C::XB + plan.y_bytes);
   if (plan.stages > C::MAXSTAGE) plan.stages = C::MAXSTAGE;
   const size_t smem = head + (size_t)plan.stages * (C::XB + plan.y_bytes);
   return note_cuda(launch_overlapped_in(2, pair_product_kernel<MODE>, dim3((unsigned)(2 * plan.pairs)), dim3(C::NTHREADS), smem,

@@ -64,6 +64,9 @@ struct PairPlan {
   int staged;              // kGrad: results pass through shared memory
 };
 
+// allow_*: the kernel's shared memory on the current device, ahead of its launch.
+template <int MODE>
+int allow_pair_product();
 template <int MODE>
 int launch_pair_product(const ProductMaps& maps, const ProductParams& p, PairPlan plan, cudaStream_t stream);
 
@@ -78,6 +81,8 @@ constexpr int kFewMaxStages = 12, kFewHead = 1024 + 256;                     // 
 constexpr int kFewSmemHalf = 113 * 1024, kFewSmemFull = 226 * 1024;          // bytes of a CTA: two per SM, one per SM
 constexpr int few_weights(int mode) { return mode == kGated16 || mode == kGatedI8 ? 2 : 1; }   // weights a tile reads per k-block
 
+template <int MODE>
+int allow_few_product();
 template <int MODE>
 int launch_few_product(const ProductMaps& maps, const ProductParams& p, const FewPlan& f, cudaStream_t stream);
 

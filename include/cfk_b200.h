@@ -162,8 +162,8 @@ int cfk_gemm_plan(const cfk_gemm_args* args, int plan[3]);
  * The lengths themselves are free: any m, n, k from 1 to 2^31 - 256 whose tiles a launch can count.  Nothing is read or written
  * behind the end of a row.  Outputs overlap no input and no other output, unless a comment allows it.  Sums are exact (integers) or fp32; results are rounded once.
  * Pointers and stream belong to the current device.  No workspace but the status block (cfk_device_status reports a wait
- * that gave up, codes 211-214 and 221-223; until it is read the products do nothing, as all tensor-core kernels here, while
- * cfk_quantize_rows and the elementwise part of the backward pass run); calls can be captured.  Results do not depend on timing.  Which kernel a call
+ * that gave up, codes 211-214 and 221-223; until it is read these calls do nothing, as all tensor-core kernels here, except
+ * cfk_quantize_rows, which runs); calls can be captured.  Results do not depend on timing.  Which kernel a call
  * runs depends on its sizes and types (and, with it, the order of fp32 sums); integer sums do not depend on it.
  */
 
@@ -230,7 +230,9 @@ int cfk_ffn_gated(const cfk_ffn_gated_args* args, cfk_stream_t stream);
  *   dx = dgate Wg + dup Wu,  dw_gate = dgate^T x,  dw_up = dup^T x.
  * dgate and dup are outputs that the products read: they are rounded to dtype, as the tensor core takes them, which adds to
  * each product an error of the size of its own rounding.  dgate may be the buffer of gate (or dup that of up) with the same
- * stride, which saves their memory.  Two or three launches; dx null leaves its product out, dw_gate and dw_up (both or neither) theirs.
+ * stride, which saves their memory; a call enqueued behind a wait that gave up leaves them as they were and can be repeated, but if a wait
+ * gives up while the call itself runs they may hold gradients already, and the forward call has to be repeated first.  Two or three
+ * launches; dx null leaves its product out, dw_gate and dw_up (both or neither) theirs.
  * act'(0) of RELU is 0.
  */
 typedef struct cfk_ffn_gated_backward_args {
