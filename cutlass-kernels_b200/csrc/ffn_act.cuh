@@ -1,4 +1,5 @@
-// The activations of the gated feed-forward block and their derivatives, in fp32.
+// Elementwise arithmetic of the feed-forward products: scales of integer sums, activations and their derivatives, in fp32.
+//
 //   SiLU x s(x), GELU_TANH x s(2a(x)) with a = sqrt(2/pi) (x + 0.044715 x^3), since (1 + tanh a) / 2 = s(2a), s the logistic
 //   function; GELU x Phi(x) with Phi(x) = erfc(-x / sqrt 2) / 2, which keeps its relative accuracy where 1 + erf would cancel.
 // With r = 2^(-|x| log2(e) / 2): s(|x|) = 1 / (1 + r^2), s(-|x|) = r^2 / (1 + r^2), by the special-function unit, whose divisor stays in
@@ -12,6 +13,15 @@
 #include "../../include/cfk_b200.h"
 
 namespace cfk {
+
+// A row's scale, which multiplies an integer sum ahead of the column's: scale = by * rest.  Beside a scale of 2^64 or more a sum could
+// pass the range of fp32 although its product with a small column scale does not, so 2^32 of it are left for the end.  (Below, a
+// sum of up to 2^31 stays under 2^95; a sum times a subnormal scale is exact or normal, so nothing is lost at the other end.)
+struct RowScale { float by, rest; };
+__device__ __forceinline__ RowScale split_row_scale(float s) {
+  const bool large = fabsf(s) >= 18446744073709551616.f;
+  return RowScale{large ? s * 2.3283064365386963e-10f : s, large ? 4294967296.f : 1.f};
+}
 
 // s(z) = d a^2
 struct Logistic { float r, d, a; };

@@ -211,13 +211,26 @@ few_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_consta
     const int token = tok0 + t0;
     float v[8], u[8];
     if constexpr (I8) {
-      const float rs = lane < n ? p.row_scale[token + lane] : 0.f;     // n <= 8
+      const RowScale rs = split_row_scale(lane < n ? p.row_scale[token + lane] : 0.f);     // n <= 8
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float rsi = __shfl_sync(0xffffffffu, rs, i);
+        const float rsi = __shfl_sync(0xffffffffu, rs.by, i);
         v[i] = __int2float_rn((int)s0[i]) * rsi * cs;
         if constexpr (GATED) u[i] = __int2float_rn((int)s1[i]) * rsi * cs2;
-        else if (p.bias != nullptr) v[i] += bias;
+      }
+      if (__any_sync(0xffffffffu, rs.rest != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float rest = __shfl_sync(0xffffffffu, rs.rest, i);
+          v[i] *= rest;
+          if constexpr (GATED) u[i] *= rest;
+        }
+      }
+      if constexpr (!GATED) {
+        if (p.bias != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] += bias;
+        }
       }
     } else {
 #pragma unroll

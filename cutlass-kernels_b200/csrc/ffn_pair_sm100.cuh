@@ -23,6 +23,8 @@
 // the 1.3 GHz that the power cap leaves: gated 8192 x 11264 x 4096 in bf16 1051 us, 1440 TFLOP/s; its 8-bit form 507 us and 8192^3
 // in 8 bits 370 us, 2980 TOP/s; the gradients of 8192 x 11264 x 4096 2300 to 2450 us, 1230 to 1310 TFLOP/s.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 #include "ffn_act.cuh"
 #include "ffn_params.h"
@@ -136,9 +138,13 @@ __device__ __forceinline__ void store_staged(const ProductParams& p, int which, 
 }
 
 // int32 sums (as bit patterns) to scaled fp32; lane i holds the scale of column i
-__device__ __forceinline__ void scale_columns(float (&v)[32], float row_scale, float col_scale) {
+template <bool REST>
+__device__ __forceinline__ void scale_columns(float (&v)[32], const RowScale& row_scale, float col_scale) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __int2float_rn(__float_as_int(v[i])) * row_scale * __shfl_sync(0xffffffffu, col_scale, i);
+  for (int i = 0; i < 32; ++i) {
+    v[i] = __int2float_rn(__float_as_int(v[i])) * row_scale.by * __shfl_sync(0xffffffffu, col_scale, i);
+    if constexpr (REST) v[i] *= row_scale.rest;
+  }
 }
 // h = act(gate) * up in place of gate
 template <int ACT>
@@ -326,69 +332,89 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
     const uint32_t stage = sStage + (warp - 2) * C::STAGEB;
     const bool staged = GRAD && plan.staged;
     const int step = staged ? 64 : 32;
-    int local = 0;
-    bool ok = true;
-    for (PairTile t; ok && pair_tile(t, plan, pair_id, local, GRAD, KB); ++local) {
+    // integer modes: this thread's row scale, read a tile ahead
+    auto row_scale = [&](const PairTile& t) {
+      const int row = t.tr * C::TM + (int)rank * C::BM + q * 32 + lane;
+      return I8 && row < t.rows ? p.row_scale[row] : 0.f;
+    };
+    PairTile t;
+    bool more = pair_tile(t, plan, pair_id, 0, GRAD, KB);
+    float next_scale = more ? row_scale(t) : 0.f;
+    for (int local = 0; more; ++local) {
       const int buf = local & 1;
       const int row0 = t.tr * C::TM + (int)rank * C::BM + q * 32, row = row0 + lane;
       const int tcols = GATED ? t.bn : 2 * t.bn, col0 = t.tc * tcols;
       const int end = t.cols - col0 < tcols ? t.cols - col0 : tcols;     // columns of the tile that exist
       const uint32_t acc = tmem_base + lane_base + buf * C::TN;
       const bool inside = row < t.rows;
-      float rs = 0.f;
-      if constexpr (I8) rs = inside ? p.row_scale[row] : 0.f;
-      ok = mbar_wait_warp(bar_acc_full + 8 * buf, (local >> 1) & 1, actx, kErrPairAccFull);
-      if (!ok) break;
+      const RowScale rs = split_row_scale(next_scale);
+      PairTile next;
+      more = pair_tile(next, plan, pair_id, local + 1, GRAD, KB);
+      if (!mbar_wait_warp(bar_acc_full + 8 * buf, (local >> 1) & 1, actx, kErrPairAccFull)) break;
       tc_fence_after_sync();
+      if (more) next_scale = row_scale(next);
+      // REST: a row of the warp has a scale with a rest.  Tested per tile and not per 32 columns, where the branch alone took 8 % of a
+      // gated call of 2048 x 8192 x 256.
+      auto columns = [&](auto rest) {
+        [[maybe_unused]] constexpr bool REST = decltype(rest)::value;
 #pragma unroll 1
-      for (int cb = grp * step; cb < end; cb += C::GROUPS * step) {
-        const int col = col0 + cb, mine = col + lane;          // this lane's column: its scales reach the others by shuffle
-        float v[32];
-        if constexpr (GATED) {
-          float u[32];
-          tmem_ld_x32(acc + cb, reinterpret_cast<uint32_t*>(v));
-          tmem_ld_x32(acc + t.bn + cb, reinterpret_cast<uint32_t*>(u));
-          if constexpr (I8) {
-            const float gs = mine < t.cols ? p.col_scale[mine] : 0.f, us = mine < t.cols ? p.col_scale2[mine] : 0.f;
+        for (int cb = grp * step; cb < end; cb += C::GROUPS * step) {
+          const int col = col0 + cb;
+          [[maybe_unused]] const int mine = col + lane;          // this lane's column: its scales reach the others by shuffle
+          float v[32];
+          if constexpr (GATED) {
+            float u[32];
+            tmem_ld_x32(acc + cb, reinterpret_cast<uint32_t*>(v));
+            tmem_ld_x32(acc + t.bn + cb, reinterpret_cast<uint32_t*>(u));
+            if constexpr (I8) {
+              const float gs = mine < t.cols ? p.col_scale[mine] : 0.f, us = mine < t.cols ? p.col_scale2[mine] : 0.f;
+              tmem_wait_ld();
+              scale_columns<REST>(v, rs, gs);
+              scale_columns<REST>(u, rs, us);
+            } else {
+              tmem_wait_ld();
+            }
+            if (p.keep && inside) {
+              store_columns(p, 1, row, col, t.cols, v);
+              store_columns(p, 2, row, col, t.cols, u);
+            }
+            gate_columns(p.act, v, u);
+            if (inside) store_columns(p, 0, row, col, t.cols, v);
+          } else if constexpr (I8) {
+            tmem_ld_x32(acc + cb, reinterpret_cast<uint32_t*>(v));
+            const float cs = mine < t.cols ? p.col_scale[mine] : 0.f;
+            const float bs = p.bias != nullptr && mine < t.cols ? p.bias[mine] : 0.f;
             tmem_wait_ld();
-            scale_columns(v, rs, gs);
-            scale_columns(u, rs, us);
-          } else {
-            tmem_wait_ld();
-          }
-          if (p.keep && inside) {
-            store_columns(p, 1, row, col, t.cols, v);
-            store_columns(p, 2, row, col, t.cols, u);
-          }
-          gate_columns(p.act, v, u);
-          if (inside) store_columns(p, 0, row, col, t.cols, v);
-        } else if constexpr (I8) {
-          tmem_ld_x32(acc + cb, reinterpret_cast<uint32_t*>(v));
-          const float cs = mine < t.cols ? p.col_scale[mine] : 0.f;
-          const float bs = p.bias != nullptr && mine < t.cols ? p.bias[mine] : 0.f;
-          tmem_wait_ld();
-          scale_columns(v, rs, cs);
-          if (p.bias != nullptr) {
+            scale_columns<REST>(v, rs, cs);
+            if (p.bias != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, bs, i);
-          }
-          if (inside) store_columns(p, 0, row, col, t.cols, v);
-        } else {
-          const int which = t.kind == 0 ? 0 : 1 + t.batch;
+              for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, bs, i);
+            }
+            if (inside) store_columns(p, 0, row, col, t.cols, v);
+          } else {
+            const int which = t.kind == 0 ? 0 : 1 + t.batch;
 #pragma unroll 1
-          for (int h = 0; h < step && cb + h < end; h += 32) {
-            tmem_ld_x32(acc + cb + h, reinterpret_cast<uint32_t*>(v));
-            tmem_wait_ld();
-            if (staged) stage_columns(stage, lane, h / 8, p.bf16, v);
-            else if (inside) store_columns(p, which, row, col, t.cols, v);
+            for (int h = 0; h < step && cb + h < end; h += 32) {
+              tmem_ld_x32(acc + cb + h, reinterpret_cast<uint32_t*>(v));
+              tmem_wait_ld();
+              if (staged) stage_columns(stage, lane, h / 8, p.bf16, v);
+              else if (inside) store_columns(p, which, row, col, t.cols, v);
+            }
+            if (staged) store_staged(p, which, stage, row0, t.rows, col, end - cb < 64 ? col0 + end : col + 64);
           }
-          if (staged) store_staged(p, which, stage, row0, t.rows, col, end - cb < 64 ? col0 + end : col + 64);
+          __syncwarp();
         }
-        __syncwarp();
+      };
+      if constexpr (I8) {
+        if (__any_sync(0xffffffffu, rs.rest != 1.f)) columns(std::true_type());
+        else columns(std::false_type());
+      } else {
+        columns(std::false_type());
       }
       // this warp has read the accumulator: the next tile but one may overwrite it
       tc_fence_before_sync();
       mbar_arrive_cluster_warp(leader_acc_empty + 8 * buf);
+      t = next;
     }
   }
 
