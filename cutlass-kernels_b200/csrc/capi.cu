@@ -30,6 +30,26 @@ cudaError_t note_cuda(cudaError_t e, const char* what) {
 static std::mutex g_mu;
 static int* g_status_block[64] = {nullptr};
 
+// Allocated and cleared apart from whatever the caller's streams do: the first call may be one that is captured, where an
+// allocation is allowed in relaxed mode only, and work on the legacy stream not at all.
+static int* allocate_status_block() {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (note_cuda(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode") != cudaSuccess) return nullptr;
+  int* p = nullptr;
+  cudaStream_t own = nullptr;
+  bool ok = note_cuda(cudaMalloc(&p, 256), "cudaMalloc(status block)") == cudaSuccess;
+  ok = ok && note_cuda(cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking), "cudaStreamCreate(status block)") == cudaSuccess;
+  ok = ok && note_cuda(cudaMemsetAsync(p, 0, 256, own), "cudaMemsetAsync(status block)") == cudaSuccess;
+  ok = ok && note_cuda(cudaStreamSynchronize(own), "cudaStreamSynchronize(status block)") == cudaSuccess;
+  if (own) (void)cudaStreamDestroy(own);
+  if (!ok && p) {
+    (void)cudaFree(p);
+    p = nullptr;
+  }
+  (void)cudaThreadExchangeStreamCaptureMode(&mode);
+  return p;
+}
+
 int* device_status_block(int* err) {
   int dev = -1;
   if (note_cuda(cudaGetDevice(&dev), "cudaGetDevice") != cudaSuccess || dev < 0 || dev >= 64) {
@@ -38,12 +58,8 @@ int* device_status_block(int* err) {
   }
   std::lock_guard<std::mutex> lk(g_mu);
   if (!g_status_block[dev]) {
-    int* p = nullptr;
-    if (note_cuda(cudaMalloc(&p, 256), "cudaMalloc(status block)") != cudaSuccess) {
-      if (err) *err = CFK_ERR_NO_DRIVER;
-      return nullptr;
-    }
-    if (note_cuda(cudaMemset(p, 0, 256), "cudaMemset(status block)") != cudaSuccess) {
+    int* p = allocate_status_block();
+    if (!p) {
       if (err) *err = CFK_ERR_NO_DRIVER;
       return nullptr;
     }
