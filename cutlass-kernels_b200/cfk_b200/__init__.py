@@ -90,8 +90,10 @@ def _ptr(x):
         return x
     try:
         return x.data_ptr()
-    except AttributeError:       # an integer of another type
-        return int(x)
+    except AttributeError:
+        if isinstance(x, int):   # a class derived from int
+            return x
+        raise
 
 
 _PACKED = (0, 0, 0)
