@@ -273,8 +273,40 @@ static int encode(CUtensorMap* map, const Matrix& m, int box_rows) {
 // Operands and results as in ProductMaps and ProductParams; unused ones have a null base.
 struct ProductCall {
   Matrix x[2], y[3], d[3];
+  Matrix elementwise[3];      // what the elementwise launch of the backward pass reads: dh, gate, up
   ProductParams p;
 };
+
+// No result shares memory with another or with what the call reads, but for a result of the elementwise launch in the very place of its
+// input.
+static bool results_apart(const ProductCall& c, bool backward) {
+  const auto span = [](const Matrix& m) {
+    const int64_t e = dtype_size(m.dtype);
+    return RowSpan{m.base, m.rows, m.cols * e, m.stride * e};
+  };
+  const auto vec = [](const float* v, int n) { return RowSpan{v, 1, 4 * (int64_t)n, 4 * (int64_t)n}; };
+  RowSpan out[5], in[8];
+  int outs = 0, ins = 0;
+  for (const Matrix& m : c.d) out[outs++] = span(m);
+  for (const Matrix& m : c.y) in[ins++] = span(m);
+  if (backward) {
+    for (const Matrix& m : c.x) out[outs++] = span(m);               // dgate, dup
+    in[ins++] = span(c.elementwise[0]);
+    for (int i = 0; i < 2; ++i)
+      if (c.elementwise[1 + i].base != c.x[i].base) in[ins++] = span(c.elementwise[1 + i]);
+  } else {
+    in[ins++] = span(c.x[0]);
+    in[ins++] = vec(c.p.row_scale, c.p.rows);
+    for (const float* v : {c.p.col_scale, c.p.col_scale2, c.p.bias}) in[ins++] = vec(v, c.p.cols);
+  }
+  for (int i = 0; i < outs; ++i) {
+    for (int j = 0; j < i; ++j)
+      if (share_memory(out[i], out[j])) return false;
+    for (int j = 0; j < ins; ++j)
+      if (share_memory(out[i], in[j])) return false;
+  }
+  return true;
+}
 
 static int prepare_results(const ProductCall& c, ProductParams* p) {
   int rc = CFK_OK;
@@ -331,12 +363,13 @@ static int prepare_pairs(const ProductCall& c, PairPlan plan, PairLaunch* l) {
 template <int MODE>
 static int run_product(const ProductCall& c, cudaStream_t stream) {
   const ProductPlan plan = plan_product(MODE, c.p.rows, c.p.cols, c.p.reduce);
+  if (plan.few.tt == 0 && too_many_tiles(plan.pair)) return CFK_ERR_UNSUPPORTED;
+  if (!results_apart(c, false)) return CFK_ERR_INVALID_ARG;
   if (plan.few.tt > 0) {
     FewLaunch l;
     const int rc = prepare_few<MODE>(c, plan.few, &l);
     return rc ? rc : launch_few_product<MODE>(l.maps, l.p, l.plan, stream);
   }
-  if (too_many_tiles(plan.pair)) return CFK_ERR_UNSUPPORTED;
   PairLaunch l;
   const int rc = prepare_pairs<MODE>(c, plan.pair, &l);
   return rc ? rc : launch_pair_product<MODE>(l.maps, l.p, l.plan, stream);
@@ -416,12 +449,14 @@ static int check_backward(const cfk_ffn_gated_backward_args* a, ProductCall* c) 
   c->d[0] = {a->dx, dt, a->m, a->k, packed(a->dx_stride, a->k)};
   c->d[1] = {a->dw_gate, dt, a->n, a->k, dw_s};
   c->d[2] = {a->dw_up, dt, a->n, a->k, dw_s};
-  const Matrix in[3] = {{a->dh, dt, a->m, a->n, packed(a->dh_stride, a->n)}, {a->gate, dt, a->m, a->n, pre_s},
-                        {a->up, dt, a->m, a->n, pre_s}};
+  Matrix* const in = c->elementwise;
+  in[0] = {a->dh, dt, a->m, a->n, packed(a->dh_stride, a->n)};
+  in[1] = {a->gate, dt, a->m, a->n, pre_s};
+  in[2] = {a->up, dt, a->m, a->n, pre_s};
   for (int i = 0; i < 3; ++i)
     if (!rows_ok(in[i]) || !rows_ok(c->y[i]) || (i < 2 && !rows_ok(c->x[i])) || (c->d[i].base && !rows_ok(c->d[i])))
       return CFK_ERR_INVALID_ARG;
-  // the only buffers that may be shared: dgate on gate, dup on up, row for row
+  // dgate may take the place of gate and dup that of up, row for row (results_apart has the rest)
   if (a->dgate == a->dup || a->dgate == a->up || a->dup == a->gate || a->dgate == a->dh || a->dup == a->dh) return CFK_ERR_INVALID_ARG;
   if ((a->dgate == a->gate || a->dup == a->up) && pre_s != dpre_s) return CFK_ERR_INVALID_ARG;
   if (!size_ok(a->m, a->n, a->k) || (long long)a->m * ((a->n + 7) / 8) > 0xffffff00LL) return CFK_ERR_UNSUPPORTED;
@@ -470,6 +505,7 @@ extern "C" int cfk_ffn_gated_backward(const cfk_ffn_gated_backward_args* a, cfk_
   if (rc) return rc;
   const ProductPlan plan = plan_backward(a);
   if (too_many_tiles(plan.pair)) return CFK_ERR_UNSUPPORTED;
+  if (!results_apart(c, true)) return CFK_ERR_INVALID_ARG;
   const int* status = device_status_block(&rc);
   if (!status) return rc;
   // in place the first launch takes the place of its inputs: nothing that could fail is left for after it but the launches

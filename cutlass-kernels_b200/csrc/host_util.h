@@ -79,6 +79,24 @@ inline bool rows_ok(const void* base, int dt, int64_t cols, int64_t stride) {
   return ((uintptr_t)base & 15u) == 0 && stride >= cols && stride < (int64_t)1 << 31 && (stride * dtype_size(dt)) % 16 == 0;
 }
 
+// Rows of a matrix in memory: `rows` of `bytes` bytes, `stride` bytes apart.
+struct RowSpan {
+  const void* base;
+  int64_t rows, bytes, stride;
+};
+// Whether two of them share memory (a null base shares none).  Finds it for matrices with the same distance of rows, as halves of a
+// wider matrix have, and for those without gaps; of others it looks at the first row of the one that begins later.
+inline bool share_memory(const RowSpan& a, const RowSpan& b) {
+  if (!a.base || !b.base) return false;
+  const bool a_first = (uintptr_t)a.base <= (uintptr_t)b.base;
+  const RowSpan &lo = a_first ? a : b, &hi = a_first ? b : a;
+  const int64_t d = (int64_t)((uintptr_t)hi.base - (uintptr_t)lo.base);
+  const int64_t row = d / lo.stride, at = d % lo.stride;           // of lo; no product of sizes, which could pass 64 bits
+  if (row >= lo.rows) return false;
+  const int64_t run = hi.stride == hi.bytes ? hi.rows : 1;         // rows that hi covers without a gap
+  return at < lo.bytes || (row + 1 < lo.rows && run > (lo.stride - at) / hi.bytes);
+}
+
 // Generic tiled descriptor.  dims/box are innermost first; strides_bytes has rank-1 entries.
 // Returns CFK_OK, CFK_ERR_NO_DRIVER or CFK_ERR_DESCRIPTOR.
 int encode_tiled(CUtensorMap* map, int dtype, int rank, const void* base, const uint64_t* dims,

@@ -166,6 +166,10 @@ extern "C" int cfk_quantize_rows(const void* src, int src_dtype, int64_t src_str
   if (dst_stride == 0) dst_stride = cols;
   if (!rows_ok(src, src_dtype, cols, src_stride) || !rows_ok(dst, CFK_INT8, cols, dst_stride) || ((uintptr_t)scale & 3u))
     return CFK_ERR_INVALID_ARG;
+  const int64_t size = dtype_size(src_dtype);
+  const RowSpan in{src, rows, cols * size, src_stride * size}, q{dst, rows, cols, dst_stride};
+  const RowSpan s{scale, 1, 4 * (int64_t)rows, 4 * (int64_t)rows};
+  if (share_memory(in, q) || share_memory(in, s) || share_memory(q, s)) return CFK_ERR_INVALID_ARG;
   const cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
   switch (src_dtype) {

@@ -160,7 +160,8 @@ int cfk_gemm_plan(const cfk_gemm_args* args, int plan[3]);
  * core reads (operands) and of every output of cfk_gemm_i8, cfk_ffn_gated and cfk_ffn_gated_backward start at multiples of 16
  * bytes: base pointers are 16-byte aligned and stride times element size is a multiple of 16, else CFK_ERR_INVALID_ARG.
  * The lengths themselves are free: any m, n, k from 1 to 2^31 - 256 whose tiles a launch can count.  Nothing is read or written
- * behind the end of a row.  Outputs overlap no input and no other output, unless a comment allows it.  Sums are exact (integers) or fp32; results are rounded once.
+ * behind the end of a row.  Outputs overlap no input and no other output, unless a comment allows it: CFK_ERR_INVALID_ARG for matrices whose
+ * rows are equally far apart (halves of a wider matrix are told from overlaps) or have no gaps between them.  Sums are exact (integers) or fp32; results are rounded once.
  * Pointers and stream belong to the current device.  No workspace but the status block (cfk_device_status reports a wait
  * that gave up, codes 211-214 and 221-223; until it is read these calls do nothing, as all tensor-core kernels here, except
  * cfk_quantize_rows, which runs); calls can be captured.  Results do not depend on timing.  Which kernel a call
