@@ -101,8 +101,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const A
 }
 // Same, with a warp-uniform answer (needed before warp-collective tcgen05.ld/st).
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, const AbortCtx& ctx, int where,
-                                               unsigned backoff_ns = 0) {
-  const bool ok = mbar_wait(bar, parity, ctx, where, kWaitLimitNs, backoff_ns);
+                                               unsigned backoff_ns = 0, unsigned long long limit_ns = kWaitLimitNs) {
+  const bool ok = mbar_wait(bar, parity, ctx, where, limit_ns, backoff_ns);
   return __all_sync(0xffffffffu, ok);
 }
 

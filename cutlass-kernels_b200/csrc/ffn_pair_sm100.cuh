@@ -350,7 +350,7 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
       const RowScale rs = split_row_scale(next_scale);
       PairTile next;
       more = pair_tile(next, plan, pair_id, local + 1, GRAD, KB);
-      if (!mbar_wait_warp(bar_acc_full + 8 * buf, (local >> 1) & 1, actx, kErrPairAccFull)) break;
+      if (!mbar_wait_warp(bar_acc_full + 8 * buf, (local >> 1) & 1, actx, kErrPairAccFull, 0, kWaitLimitNs + t.nkb * kNsPerBlock)) break;
       tc_fence_after_sync();
       if (more) next_scale = row_scale(next);
       // REST: a row of the warp has a scale with a rest.  Tested per tile and not per 32 columns, where the branch alone took 8 % of a

@@ -6,6 +6,10 @@
 
 namespace cfk {
 
+// Limit of the wait for an accumulator, which lasts as long as its reduction: 1 us per k-block on top of the limit of other waits, where
+// a k-block takes 0.15 to 0.3 us.  A tile of 900 million tokens' weight gradients takes 3 s.
+constexpr unsigned long long kNsPerBlock = 1000;
+
 // What a kernel computes; `tokens` and `channels` are the rows of activations and of weights.
 enum ProductMode {
   kProductI8 = 0,   // C = scaled (A B^T), 8-bit integers
