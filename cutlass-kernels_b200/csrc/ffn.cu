@@ -315,7 +315,7 @@ static int prepare_results(const ProductCall& c, ProductParams* p) {
   for (int i = 0; i < 3; ++i) {
     p->d[i] = const_cast<void*>(c.d[i].base);
     p->d_stride[i] = c.d[i].stride;
-    if (((uintptr_t)p->d[i] | (uintptr_t)(c.d[i].stride * dtype_size(c.d[i].dtype))) & 31u) p->wide = 0;
+    if (p->d[i] && (((uintptr_t)p->d[i] | (uintptr_t)(c.d[i].stride * dtype_size(c.d[i].dtype))) & 31u)) p->wide = 0;
   }
   return rc;
 }

@@ -34,7 +34,7 @@ struct ProductParams {
   const float* bias;       // kProductI8, or null
   void* d[3];              // results (kGated*: h, gate, up; kGrad: dx, dw_gate, dw_up) and the distance of their rows
   int64_t d_stride[3];
-  int wide;                // all rows of the results start at multiples of 32 bytes
+  int wide;                // all rows of the results that exist start at multiples of 32 bytes
   int* status;
 };
 
