@@ -84,9 +84,11 @@ static cudaError_t launch_gate_grad(const cfk_ffn_gated_backward_args* a, const 
 }
 
 // ---- cuts -------------------------------------------------------------------------------------------------------------------
-// Which kernel and which tiles follows from estimates of its time, in us, whose constants are fits to a sweep of 1170 calls (1 to 16000
-// tokens, widths 128 to 16384 and 8192) x all cuts: root mean square error 8 to 15 %.  The cut they choose is 1 to 4 % slower than the
-// best one measured, on average over the calls of a kind, and 31 % at worst.
+// Which kernel and which tiles follows from estimates of its time, in us.  Their constants are coefficients of terms that overlap, not
+// rates that a part of the chip reaches: fits (root mean square error 8 to 15 %) to a sweep of 1170 calls, 1 to 16000 tokens and
+// widths 128 to 16384 and 8192, from before tiles of 48, 96 and 192 tokens existed.  With those, over 1440 calls of 1 to 3000 tokens x all
+// cuts that now exist, the cut they choose is slower than the best one measured by 0.5 % (dw) to 2.8 % (8-bit products) on average over
+// the calls of a kind, and by 38 % at worst (45 % in a backward call of 88 tokens, where dx went to the kernel for few).
 constexpr int kPairs = kSMs / 2;
 
 static bool is_gated(int mode) { return mode == kGated16 || mode == kGatedI8; }

@@ -14,9 +14,12 @@
 //              ([accumulator][token][channel], the ring is free by then); after a cluster barrier each finishes its share of the
 //              tokens, adding the parts in order through distributed shared memory.  Nothing depends on timing.
 //
-// Bound by DRAM once the first k-blocks have arrived, 2.6 us after the start: one token through the gated 11264 x 4096 in bf16 takes 32 us
-// (184.6 MB, 5.8 TB/s), 16 tokens in 8 bits 17.5 us; 48 tokens of 4096 x 11264 in 8 bits 13 us, of which 2 to 3 are the exchange of the
-// split.  An SM takes in at most about 110 KB/us (85 of MN-major k-blocks), so few tiles split their reduction.
+// Bound by DRAM once the first k-blocks have arrived, 2.6 us after the start.  Replayed from a graph: one token through the gated 11264 x
+// 4096 in bf16 32 to 33 us (184.6 MB, 5.6 to 5.8 TB/s), 16 tokens in 8 bits 17.5 to 18 us; 48 tokens of 4096 x 11264 in 8 bits 13 us, of which
+// 2 to 3 are the exchange of the split.  (As calls of the Python binding 35 to 36, 19.4 and 14 us.)
+// A CTA alone on its SM takes a round of 0.19 us per k-block of a product, 0.23 of a gated tile and 0.24 of MN-major weights, with 16 tokens
+// or 128: 94 to 168, 148 to 209 and 76 to 141 KB/us.  148 of them get 7.6 TB/s of weights with 16 tokens, and with 128, whose
+// re-reads come from L2, 13 TB/s (gated 9.8).  So few tiles split their reduction: one CTA per SM, or a few more, fetch what there is.
 //
 // Shared memory is sized so that two CTAs fit on an SM where three stages fit in half of it.  Tensor memory never takes a larger
 // share of an SM than shared memory does, so residents cannot run out of columns: tcgen05.alloc, which waits without a limit, never

@@ -20,8 +20,9 @@
 // A tile is 2 bn accumulator columns wide, bn = 128, 96 or 64 by what fills the last wave of pairs best (ffn.cu).  Bound by the tensor
 // core: 512 clk of MMA per k-block of 128 bytes at bn = 128 against 32 KB of loads per SM and, in the gated modes, an epilogue of
 // two special-function operations per element of h that runs beside the next tile's main loop.  The pipe is 88 to 96 % active, at
-// the 1.3 GHz that the power cap leaves: gated 8192 x 11264 x 4096 in bf16 1051 us, 1440 TFLOP/s; its 8-bit form 507 us and 8192^3
-// in 8 bits 370 us, 2980 TOP/s; the gradients of 8192 x 11264 x 4096 2300 to 2450 us, 1230 to 1310 TFLOP/s.
+// the 1.15 to 1.3 GHz that the power cap leaves, and the range between boxes is wide: gated 8192 x 11264 x 4096 in bf16 1051 to 1121 us, 1350
+// to 1440 TFLOP/s; its 8-bit form 507 to 553 us; 8192^3 in 8 bits 334 us (3290 TOP/s) for a few launches and 370 to 413 (2660 to 2970) for
+// seconds on end; the gradients of 8192 x 11264 x 4096 2300 to 2790 us, 1080 to 1310 TFLOP/s.
 #pragma once
 #include <type_traits>
 

@@ -160,12 +160,14 @@ int cfk_gemm_plan(const cfk_gemm_args* args, int plan[3]);
  * core reads (operands) and of every output of cfk_gemm_i8, cfk_ffn_gated and cfk_ffn_gated_backward start at multiples of 16
  * bytes: base pointers are 16-byte aligned and stride times element size is a multiple of 16, else CFK_ERR_INVALID_ARG.
  * The lengths themselves are free: any m, n, k from 1 to 2^31 - 256 whose tiles a launch can count.  Nothing is read or written
- * behind the end of a row.  Outputs overlap no input and no other output, unless a comment allows it: CFK_ERR_INVALID_ARG for matrices whose
- * rows are equally far apart (halves of a wider matrix are told from overlaps) or have no gaps between them.  Sums are exact (integers) or fp32; results are rounded once.
+ * behind the end of a row.  Outputs overlap no input and no other output, unless a comment allows it: CFK_ERR_INVALID_ARG for
+ * matrices whose rows are equally far apart (halves of a wider matrix are told from overlaps) or have no gaps between them.
+ * Sums of 16-bit products are fp32.  Integer sums are exact, and are scaled in fp32: the sum (rounded above 2^24) times the row's scale,
+ * times the column's, plus the bias.  Results are rounded once more, to their type.
  * Pointers and stream belong to the current device.  No workspace but the status block (cfk_device_status reports a wait
  * that gave up, codes 211-214 and 221-223; until it is read these calls do nothing, as all tensor-core kernels here, except
- * cfk_quantize_rows, which runs); calls can be captured.  Results do not depend on timing.  Which kernel a call
- * runs depends on its sizes and types (and, with it, the order of fp32 sums); integer sums do not depend on it.
+ * cfk_quantize_rows, which runs).  Calls can be captured, the first one on a device too.  Results do not depend on timing.  Which
+ * kernel a call runs depends on its sizes and types (and, with it, the order of fp32 sums); integer sums do not depend on it.
  */
 
 /*
@@ -180,7 +182,7 @@ int cfk_quantize_rows(const void* src, int src_dtype, int64_t src_stride, void* 
 
 /*
  * C[i][j] = a_scale[i] * b_scale[j] * sum_k A[i][k] B[j][k]  (+ bias[j]), A [m][k] and B [n][k] signed 8-bit integers.
- * The sums are 32-bit integers and exact; k above 131071 (2^31 / 128^2) is refused, CFK_ERR_UNSUPPORTED.
+ * The sums are 32-bit integers and exact (a result that fp32 holds is found whatever the sizes of the two scales); k above 131071 (2^31 / 128^2) is refused, CFK_ERR_UNSUPPORTED.
  */
 typedef struct cfk_gemm_i8_args {
   int out_dtype;               /* C: FP16, BF16 or FP32 */
@@ -202,7 +204,9 @@ enum cfk_activation { CFK_ACT_SILU = 0, CFK_ACT_GELU = 1, CFK_ACT_GELU_TANH = 2,
 /*
  * Gated feed-forward block up to its product, in one kernel:
  *   gate = x Wg^T,  up = x Wu^T,  h = act(gate) * up.
- * The projection back is a cfk_gemm or cfk_gemm_i8 of h.  Weights that are stored as one [2n][k] matrix are passed as two
+ * The projection back is a cfk_gemm_i8 or cfk_gemm of h.  cfk_gemm takes packed rows and multiples of 8 for all three sizes: for others,
+ * give h (and the gradient of it) m rounded up to 8 rows and a row distance of n rounded up to 8, zeros in what is added, which
+ * stays as it is, and the weight zeros likewise.  Weights that are stored as one [2n][k] matrix are passed as two
  * pointers into it.  With gate and up given (both or neither) the pre-activations are written too, as the backward pass
  * needs them; h is computed from the unrounded ones.
  */
