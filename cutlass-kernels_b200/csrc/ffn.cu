@@ -329,6 +329,7 @@ struct PairLaunch { ProductMaps maps; ProductParams p; PairPlan plan; };
 template <int MODE>
 static int prepare_few(const ProductCall& c, const FewPlan& few, FewLaunch* l) {
   l->p = c.p;
+  l->p.acc_limit = kWaitLimitNs + kNsPerBlock * (unsigned long long)(k_blocks(MODE, c.p.reduce) * (MODE == kGrad ? 2 : 1));
   l->plan = few;
   std::memset(&l->maps, 0, sizeof(l->maps));
   int rc = prepare_results(c, &l->p);
@@ -351,7 +352,13 @@ static int prepare_pairs(const ProductCall& c, PairPlan plan, PairLaunch* l) {
     j.per_band = make_divisor((uint32_t)(kGemmBand * j.tiles_c));
     j.tail_rows = make_divisor((uint32_t)(j.tiles_r % kGemmBand ? j.tiles_r % kGemmBand : 1));
   }
+  int longest = 0;                   // k-blocks of a tile
+  for (int i = 0; i < plan.jobs; ++i) {
+    const int n = k_blocks(MODE, plan.job[i].reduce) * (MODE == kGrad && plan.job[i].kind == 0 ? 2 : 1);
+    if (n > longest) longest = n;
+  }
   l->p = c.p;
+  l->p.acc_limit = kWaitLimitNs + kNsPerBlock * (unsigned long long)longest;
   l->plan = plan;
   std::memset(&l->maps, 0, sizeof(l->maps));
   int rc = prepare_results(c, &l->p);

@@ -205,7 +205,7 @@ few_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_consta
         else if (p.bias != nullptr) bias = p.bias[ch];
       }
     }
-    done = mbar_wait_warp(bar_acc, 0, actx, kErrFewAcc, 0, kWaitLimitNs + (kb1 - kb0) * kNsPerBlock);
+    done = mbar_wait_warp(bar_acc, 0, actx, kErrFewAcc, 0, p.acc_limit);
     tc_fence_after_sync();
   }
 

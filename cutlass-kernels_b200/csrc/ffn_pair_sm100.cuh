@@ -333,27 +333,18 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
     const uint32_t stage = sStage + (warp - 2) * C::STAGEB;
     const bool staged = GRAD && plan.staged;
     const int step = staged ? 64 : 32;
-    // integer modes: this thread's row scale, read a tile ahead
-    auto row_scale = [&](const PairTile& t) {
-      const int row = t.tr * C::TM + (int)rank * C::BM + q * 32 + lane;
-      return I8 && row < t.rows ? p.row_scale[row] : 0.f;
-    };
-    PairTile t;
-    bool more = pair_tile(t, plan, pair_id, 0, GRAD, KB);
-    float next_scale = more ? row_scale(t) : 0.f;
-    for (int local = 0; more; ++local) {
+    // One tile; false: its accumulator did not come.  `ahead` runs once it has.
+    auto finish_tile = [&](const PairTile& t, int local, float row_scale, auto ahead) {
       const int buf = local & 1;
       const int row0 = t.tr * C::TM + (int)rank * C::BM + q * 32, row = row0 + lane;
       const int tcols = GATED ? t.bn : 2 * t.bn, col0 = t.tc * tcols;
       const int end = t.cols - col0 < tcols ? t.cols - col0 : tcols;     // columns of the tile that exist
       const uint32_t acc = tmem_base + lane_base + buf * C::TN;
       const bool inside = row < t.rows;
-      const RowScale rs = split_row_scale(next_scale);
-      PairTile next;
-      more = pair_tile(next, plan, pair_id, local + 1, GRAD, KB);
-      if (!mbar_wait_warp(bar_acc_full + 8 * buf, (local >> 1) & 1, actx, kErrPairAccFull, 0, kWaitLimitNs + t.nkb * kNsPerBlock)) break;
+      [[maybe_unused]] const RowScale rs = split_row_scale(row_scale);
+      if (!mbar_wait_warp(bar_acc_full + 8 * buf, (local >> 1) & 1, actx, kErrPairAccFull, 0, p.acc_limit)) return false;
       tc_fence_after_sync();
-      if (more) next_scale = row_scale(next);
+      ahead();
       // REST: a row of the warp has a scale with a rest.  Tested per tile and not per 32 columns, where the branch alone took 8 % of a
       // gated call of 2048 x 8192 x 256.
       auto columns = [&](auto rest) {
@@ -415,7 +406,27 @@ pair_product_kernel(const __grid_constant__ ProductMaps maps, const __grid_const
       // this warp has read the accumulator: the next tile but one may overwrite it
       tc_fence_before_sync();
       mbar_arrive_cluster_warp(leader_acc_empty + 8 * buf);
-      t = next;
+      return true;
+    };
+    int local = 0;
+    if constexpr (I8) {                // this thread's row scale is read a tile ahead: the first columns wait for it (REST)
+      auto row_scale = [&](const PairTile& t) {
+        const int row = t.tr * C::TM + (int)rank * C::BM + q * 32 + lane;
+        return row < t.rows ? p.row_scale[row] : 0.f;
+      };
+      PairTile t;
+      bool more = pair_tile(t, plan, pair_id, 0, GRAD, KB);
+      float scale = more ? row_scale(t) : 0.f;
+      for (; more; ++local) {
+        const float now = scale;
+        PairTile next = t;
+        more = pair_tile(next, plan, pair_id, local + 1, GRAD, KB);
+        if (!finish_tile(t, local, now, [&] { if (more) scale = row_scale(next); })) break;
+        t = next;
+      }
+    } else {
+      bool ok = true;
+      for (PairTile t; ok && pair_tile(t, plan, pair_id, local, GRAD, KB); ++local) ok = finish_tile(t, local, 0.f, [] {});
     }
   }
 

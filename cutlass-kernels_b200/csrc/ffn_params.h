@@ -6,10 +6,6 @@
 
 namespace cfk {
 
-// Limit of the wait for an accumulator, which lasts as long as its reduction: 1 us per k-block on top of the limit of other waits, where
-// a k-block takes 0.15 to 0.3 us.  A tile of 900 million tokens' weight gradients takes 3 s.
-constexpr unsigned long long kNsPerBlock = 1000;
-
 // What a kernel computes; `tokens` and `channels` are the rows of activations and of weights.
 enum ProductMode {
   kProductI8 = 0,   // C = scaled (A B^T), 8-bit integers
@@ -36,7 +32,11 @@ struct ProductParams {
   int64_t d_stride[3];
   int wide;                // all rows of the results that exist start at multiples of 32 bytes
   int* status;
+  unsigned long long acc_limit;      // of the wait for an accumulator, ns
 };
+// An accumulator takes as long as its reduction: 1 us per k-block on top of the limit of other waits, where a k-block takes 0.15 to
+// 0.4 us.  A tile of 900 million tokens' weight gradients takes 3 s.
+constexpr unsigned long long kNsPerBlock = 1000;
 
 // Division of 0 <= n < 2^31 by a constant of the launch: a product and a shift (T. Granlund, P. Montgomery, Division by invariant
 // integers using multiplication, 1994).

@@ -1,6 +1,4 @@
 """Reductions that take longer than the two seconds that other waits of the kernels have."""
-import math
-
 import pytest
 import torch
 
@@ -35,8 +33,9 @@ def test_weight_gradients_of_900_million_tokens(lib, cuda):
     dg, du, xs = gate[at].double(), up[at].double(), rows["x"].double()
     value, slope = activation64(cfk.ACT_SILU, rows["gate"].double())
     check(du, rows["dh"].double() * value, (half(cfk.FP16) + 1e-5) * (rows["dh"].double() * value).abs() + TINY[cfk.FP16])
+    del dh, gate, up, x
+    torch.cuda.empty_cache()
     for got, d in ((dwg, dg), (dwu, du)):
         want = d.T @ xs
         e = len(at) * 2.0 ** -23 * (d.abs().T @ xs.abs())
         check(got, want, e + half(cfk.FP16) * (want.abs() + e) + TINY[cfk.FP16])
-    assert math.isfinite(float(dwg.double().sum()))
