@@ -17,18 +17,19 @@ static int64_t packed(int64_t stride, int cols) { return stride == 0 ? cols : st
 
 // dgate = dh * up * act'(gate), dup = dh * act(gate).  Memory bound: three 16-bit values in, two out, 16 bytes per access, a thread
 // reads its elements of all three before it writes, so the results may take the place of gate and up.  8192 x 11264 bf16, replayed from
-// a graph: SiLU 138 us, 6.7 TB/s, six blocks per SM (five: 146); GELU 230, its erfc.
-// Behind a wait that gave up it writes nothing, as the products that follow it: in place it would take the inputs of a repeated call.
-// The status word is read beside the elements, so the test costs a barrier and not a memory latency.
-template <int DT, int ACT>
-__global__ void __launch_bounds__(256, 6) gate_grad_kernel(const uint16_t* dh, const uint16_t* gate, const uint16_t* up, uint16_t* dgate,
-                                                        uint16_t* dup, int64_t dh_stride, int64_t pre_stride,
-                                                        int64_t dpre_stride, int cols, uint32_t nvec, uint32_t total,
-                                                        const int* status) {
+// a graph: SiLU 134 us, 6.9 TB/s, in place 140, with six blocks per SM (five: 146); GELU 228, its erfc.
+// IN_PLACE: behind a wait that gave up nothing is written, as by the products that follow, since it would overwrite the inputs of the
+// call when it is repeated.  The word is read beside the elements, so the test costs a barrier and not a memory latency: 0.5 us of 777 x
+// 2731.  (Every thread reading it: 146 us for the 140 above.)
+template <int DT, int ACT, bool IN_PLACE>
+__global__ void __launch_bounds__(256, 6)
+gate_grad_kernel(const uint16_t* dh, const uint16_t* gate, const uint16_t* up, uint16_t* dgate, uint16_t* dup, int64_t dh_stride,
+                 int64_t pre_stride, int64_t dpre_stride, int cols, uint32_t nvec, uint32_t total, const int* status) {
   grid_dependency_launch();
   grid_dependency_wait();
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
   const bool exists = idx < total;
+  if (!IN_PLACE && !exists) return;
   const uint32_t row = exists ? idx / nvec : 0u;
   const int col = exists ? (int)(idx - row * nvec) * 8 : cols;
   dh += row * dh_stride + col;
@@ -51,7 +52,7 @@ __global__ void __launch_bounds__(256, 6) gate_grad_kernel(const uint16_t* dh, c
       u.h[i] = in ? up[i] : (uint16_t)0;
     }
   }
-  if (cta_should_skip(status)) return;
+  if (IN_PLACE && cta_should_skip(status)) return;
   float x[8], y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -71,13 +72,14 @@ __global__ void __launch_bounds__(256, 6) gate_grad_kernel(const uint16_t* dh, c
   }
 }
 
-template <int DT>
+template <int DT, bool IN_PLACE>
 static cudaError_t launch_gate_grad(const cfk_ffn_gated_backward_args* a, const int* status, cudaStream_t st) {
   const int64_t dh_s = packed(a->dh_stride, a->n), pre_s = packed(a->pre_stride, a->n), dpre_s = packed(a->dpre_stride, a->n);
   const uint32_t nvec = (uint32_t)((a->n + 7) / 8), total = (uint32_t)a->m * nvec;
-  auto kern = a->activation == CFK_ACT_SILU ? gate_grad_kernel<DT, CFK_ACT_SILU>
-              : a->activation == CFK_ACT_GELU ? gate_grad_kernel<DT, CFK_ACT_GELU>
-              : a->activation == CFK_ACT_GELU_TANH ? gate_grad_kernel<DT, CFK_ACT_GELU_TANH> : gate_grad_kernel<DT, CFK_ACT_RELU>;
+  auto kern = a->activation == CFK_ACT_SILU ? gate_grad_kernel<DT, CFK_ACT_SILU, IN_PLACE>
+              : a->activation == CFK_ACT_GELU ? gate_grad_kernel<DT, CFK_ACT_GELU, IN_PLACE>
+              : a->activation == CFK_ACT_GELU_TANH ? gate_grad_kernel<DT, CFK_ACT_GELU_TANH, IN_PLACE>
+                                                   : gate_grad_kernel<DT, CFK_ACT_RELU, IN_PLACE>;
   return launch_overlapped(kern, dim3((total + 255u) / 256u), dim3(256), 0, st, (const uint16_t*)a->dh, (const uint16_t*)a->gate,
                            (const uint16_t*)a->up, (uint16_t*)a->dgate, (uint16_t*)a->dup, dh_s, pre_s, dpre_s, a->n, nvec, total,
                            status);
@@ -523,8 +525,10 @@ extern "C" int cfk_ffn_gated_backward(const cfk_ffn_gated_backward_args* a, cfk_
   if (plan.few.tt > 0 && (rc = prepare_few<kGrad>(c, plan.few, &few))) return rc;
   if (plan.pair.jobs > 0 && (rc = prepare_pairs<kGrad>(c, plan.pair, &pair))) return rc;
   const cudaStream_t st = (cudaStream_t)stream;
-  const cudaError_t e = a->dtype == CFK_FP16 ? launch_gate_grad<CFK_FP16>(a, status, st) : launch_gate_grad<CFK_BF16>(a, status, st);
-  if (note_cuda(e, "gate gradient launch") != cudaSuccess) return CFK_ERR_LAUNCH;
+  const bool in_place = a->dgate == a->gate || a->dup == a->up;
+  const auto launch = a->dtype == CFK_FP16 ? (in_place ? launch_gate_grad<CFK_FP16, true> : launch_gate_grad<CFK_FP16, false>)
+                                           : (in_place ? launch_gate_grad<CFK_BF16, true> : launch_gate_grad<CFK_BF16, false>);
+  if (note_cuda(launch(a, status, st), "gate gradient launch") != cudaSuccess) return CFK_ERR_LAUNCH;
   if (plan.few.tt > 0 && (rc = launch_few_product<kGrad>(few.maps, few.p, few.plan, st))) return rc;
   return plan.pair.jobs > 0 ? launch_pair_product<kGrad>(pair.maps, pair.p, pair.plan, st) : CFK_OK;
 }

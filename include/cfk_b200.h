@@ -166,7 +166,7 @@ int cfk_gemm_plan(const cfk_gemm_args* args, int plan[3]);
  * times the column's, plus the bias.  Results are rounded once more, to their type.
  * Pointers and stream belong to the current device.  No workspace but the status block (cfk_device_status reports a wait
  * that gave up, codes 211-214 and 221-223; until it is read these calls do nothing, as all tensor-core kernels here, except
- * cfk_quantize_rows, which runs).  Calls can be captured, the first one on a device too.  Results do not depend on timing.  Which
+ * cfk_quantize_rows and the elementwise part of a backward call that is not in place, which run).  Calls can be captured, the first one on a device too.  Results do not depend on timing.  Which
  * kernel a call runs depends on its sizes and types (and, with it, the order of fp32 sums); integer sums do not depend on it.
  */
 
